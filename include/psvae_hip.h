@@ -41,6 +41,10 @@ extern "C" {
 #define PSVAE_ACT_NONE 0
 #define PSVAE_ACT_RELU 1
 
+#define PSVAE_F32 0            /* element types of the operators that take several     */
+#define PSVAE_BF16 1
+#define PSVAE_F16 2
+
 int psvae_version(void);
 const char *psvae_last_error(void);
 
@@ -518,6 +522,83 @@ int psvae_piece_draw(int B, int V, const float *logits, int64_t ld_logits, float
                      int64_t ld_uniforms, int pad_idx, int end_idx, int first_step, const int32_t *piece_atoms,
                      int max_atom_num, int max_pos, uint8_t *active, int32_t *atoms, int32_t *length,
                      int64_t *out, int64_t ld_out, int64_t *cur, void *stream);
+
+/* ------------------------------------------------------------------------------------
+ * Between the vocabulary layer and the next token: penalties for tokens of the past, a bias, a
+ * temperature and a grammar's mask over the logits of a language model (the general form of the
+ * masks and the temperature of src/modules/vae_piece_decoder.py:139-146).  Row r = (b, t),
+ * b < B sequences, t < T positions, of logits [B, T, V] (types PSVAE_F32 / BF16 / F16):
+ *   c_i = #{j < len_r : history[b][j] == i},  len_r = history_len[r or b] (null: L; cut to 0 .. L)
+ *   a_i = l_i;  where c_i > 0:  a_i = (l_i > 0 ? l_i / repetition_b : l_i * repetition_b)
+ *                                     - frequency_b c_i - presence_b
+ *   y_i = (a_i + bias_i) / temperature_b  where bit i of the row's mask is set, else -inf
+ * Ids of the history outside 0 .. V-1 count for nothing.  What a masked logit holds (NaN,
+ * infinities) is never looked at.  A repetition or temperature read from the device that is not positive
+ * and finite makes the values that it touches NaN.
+ * The mask row is allowed[s] with s = state[r or b]; s < 0: every token, s >= S: none; without
+ * states row 0 (S == 1) or row b (S == B).  Bit i is bit i % 32 of word i / 32.
+ * ---------------------------------------------------------------------------------- */
+typedef struct psvae_shaping {
+    int B, T, V, dtype;
+    const void *logits;             /* element (b, t, i) at b * ld_b + t * ld_t + i              */
+    int64_t ld_b, ld_t;
+    const int64_t *history;         /* [B, L], rows ld_history apart; null: no penalties         */
+    int64_t ld_history;
+    int L;
+    const int32_t *history_len;     /* [B], or [B, T] when len_per_row; null: L                  */
+    int len_per_row;
+    const float *repetition_rows, *presence_rows, *frequency_rows, *temperature_rows;   /* [B], or null: */
+    float repetition, presence, frequency, temperature;                                  /* one for all   */
+    const float *bias;              /* [V] (ld_bias 0) or [B, V]; null: none                     */
+    int64_t ld_bias;
+    const int32_t *allowed;         /* [S, >= (V + 31) / 32] words; null: everything             */
+    int64_t ld_allowed;
+    int S;
+    const int32_t *state;           /* [B], or [B, T] when state_per_row; null: see above        */
+    int state_per_row;
+} psvae_shaping;
+
+/* out[r] = y (the logits' type, rounded once), rows ld_out apart.  May be the logits themselves. */
+int psvae_shape_logits_fwd(const psvae_shaping *shaping, void *out, int64_t ld_out, void *stream);
+/* dlogits[r] = g[r] * dy/dl (0 where masked); g: element (b, t, i) at b * ld_gb + t * ld_gt + i, type of the logits. */
+int psvae_shape_logits_bwd(const psvae_shaping *shaping, const void *g, int64_t ld_gb, int64_t ld_gt,
+                           void *dlogits, int64_t ld_dlogits, void *stream);
+
+/* log_prob[r] = y_tok - logsumexp(y), tok = tokens[r] (float32; a tok outside 0 .. V-1: 0 and no
+ * gradient; a masked tok, or a row that allows nothing: -inf); stats [R, 2] (maximum, sum of exponentials)
+ * is what the backward needs:  dlogits = g[r] ([i == tok] - exp(y_i - max) / sum) dy_i/dl_i
+ * (all 0 for a row that allows nothing). */
+size_t psvae_shaped_log_prob_workspace_bytes(const psvae_shaping *shaping);
+int psvae_shaped_log_prob_fwd(const psvae_shaping *shaping, const int64_t *tokens, float *log_prob, float *stats,
+                              void *workspace, size_t workspace_bytes, void *stream);
+int psvae_shaped_log_prob_bwd(const psvae_shaping *shaping, const int64_t *tokens, const float *stats, const float *g,
+                              void *dlogits, int64_t ld_dlogits, void *stream);
+
+/* One token per sequence (T == 1) from softmax(y), in 64-bit arithmetic:
+ *   tokens[b] = min(#{i : cdf_i <= uniforms[b * ld_uniforms] * cdf_last}, last i of positive probability)
+ * and its log-probability.  A row that allows nothing: empty_token and -inf; one that holds NaN or
+ * +inf where it allows it: empty_token and NaN. */
+size_t psvae_shaped_draw_workspace_bytes(const psvae_shaping *shaping);
+int psvae_shaped_draw(const psvae_shaping *shaping, const float *uniforms, int64_t ld_uniforms, int64_t empty_token,
+                      int64_t *tokens, float *log_prob, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------------------------
+ * Global-norm clipping over many tensors (torch.nn.utils.clip_grad_norm_ as the Trainer calls it,
+ * src/train.py:47), for gradients that do not sit in one flat float32 buffer.  Lists are HOST arrays of n
+ * entries, read before the call returns: device pointers, element counts (0 allowed) and types
+ * (PSVAE_F32 / BF16 / F16).
+ *   norm = sqrt(sum of squares), squares and sums in 64 bits, in an order that only the counts decide;
+ *   out_i = grad_i * min(1, max_norm / (norm + 1e-6))  (a NaN norm makes every value NaN)
+ * out_i may be grad_i itself (then a factor of 1 writes nothing) and may be of another type; otherwise no
+ * output may overlap a gradient or another output.
+ * ---------------------------------------------------------------------------------- */
+size_t psvae_grad_norm_workspace_bytes(int n, const int64_t *numel_host);
+int psvae_grad_norm(int n, const void *const *grads_host, const int64_t *numel_host, const int32_t *types_host,
+                    float *norm, void *workspace, size_t workspace_bytes, void *stream);
+int psvae_clip_grads(int n, const void *const *grads_host, const int64_t *numel_host, const int32_t *types_host,
+                     void *const *out_host, const int32_t *out_types_host, float max_norm, float *norm,
+                     void *workspace, size_t workspace_bytes, void *stream);
+
 
 /* ------------------------------------------------------------------------------------
  * Candidate atom pairs of generated molecules (src/modules/vae_piece_decoder.py:213-222): for molecule b

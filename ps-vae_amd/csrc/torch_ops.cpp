@@ -14,7 +14,9 @@
 #include <initializer_list>
 #include <map>
 #include <mutex>
+#include <tuple>
 #include <utility>
+#include <vector>
 
 #include "../../include/psvae_hip.h"
 
@@ -532,6 +534,230 @@ void gru_seq_bwd(const Tensor &gates, const Tensor &ghn, const Tensor &hall, con
                             const_cast<float *>(f32c(dgh, fn)), const_cast<float *>(f32c(dh0, fn)), cur_stream(dgi)), fn);
 }
 
+// ---- shaped logits (psvae_shaping): the description is filled from the tensors of one call
+int elem_type(const Tensor &t, const char *what) {
+    TORCH_CHECK(t.is_cuda(), what, ": psvae operators need GPU tensors (there is no CPU fallback)");
+    switch (t.scalar_type()) {
+        case at::kFloat: return PSVAE_F32;
+        case at::kBFloat16: return PSVAE_BF16;
+        case at::kHalf: return PSVAE_F16;
+        default: TORCH_CHECK(false, what, ": expected float32, bfloat16 or float16, got ", t.scalar_type());
+    }
+}
+const Tensor *given(const OptTensor &t) { return t.has_value() && t->defined() ? &*t : nullptr; }
+const int64_t *i64_rows(const Tensor &t, const char *what) {
+    TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kLong && (t.size(-1) <= 1 || t.stride(-1) == 1), what,
+                ": expected an int64 GPU tensor with contiguous rows");
+    return t.const_data_ptr<int64_t>();
+}
+
+// rows: [B] or [B, T] values of a call over B sequences of T positions; whether there is one for each row
+bool per_row(const Tensor &t, int64_t B, int64_t T, int64_t dims, const char *what, const char *name) {
+    TORCH_CHECK((t.dim() == 1 && t.size(0) == B) || (dims == 3 && t.dim() == 2 && t.size(0) == B && t.size(1) == T), what, ": ", name,
+                " must be [B]", dims == 3 ? " or [B, T]" : "", " of the logits, got ", t.sizes());
+    return t.dim() == 2;
+}
+
+struct ShapingArgs {
+    const Tensor &logits;
+    const OptTensor &history, &history_len, &repetition, &presence, &frequency, &temperature, &bias, &allowed, &state;
+    at::ArrayRef<double> scalars;   // repetition, presence, frequency, temperature where no tensor is given
+};
+
+psvae_shaping shaping_of(const ShapingArgs &a, const char *fn) {
+    const Tensor &x = a.logits;
+    TORCH_CHECK(x.dim() == 2 || x.dim() == 3, fn, ": logits must be [B, V] or [B, T, V], got ", x.sizes());
+    TORCH_CHECK(x.size(-1) >= 1 && (x.size(-1) == 1 || x.stride(-1) == 1), fn, ": logits need contiguous rows of at least one value");
+    TORCH_CHECK(a.scalars.size() == 4, fn, ": four scalars");
+    const int64_t dims = x.dim(), B = x.size(0), T = dims == 3 ? x.size(1) : 1, V = x.size(-1);
+    TORCH_CHECK(B * T < (1ll << 31) && V <= (1ll << 30), fn, ": ", B, " x ", T, " rows of ", V, " logits");
+    psvae_shaping s{};
+    s.B = T == 0 ? 0 : (int)B, s.T = T == 0 ? 1 : (int)T, s.V = (int)V, s.dtype = elem_type(x, fn);
+    s.logits = x.const_data_ptr(), s.ld_b = x.stride(0), s.ld_t = dims == 3 ? x.stride(1) : 0;
+    auto row_values = [&](const OptTensor &t, const char *name) -> const float * {
+        const Tensor *v = given(t);
+        if (!v) return nullptr;
+        TORCH_CHECK(v->is_cuda() && v->scalar_type() == at::kFloat && v->is_contiguous() && v->dim() == 1 && v->size(0) == B, fn, ": ", name,
+                    " must be a number or a contiguous float32 GPU tensor [B]");
+        return v->const_data_ptr<float>();
+    };
+    s.repetition_rows = row_values(a.repetition, "repetition"), s.presence_rows = row_values(a.presence, "presence");
+    s.frequency_rows = row_values(a.frequency, "frequency"), s.temperature_rows = row_values(a.temperature, "temperature");
+    s.repetition = (float)a.scalars[0], s.presence = (float)a.scalars[1], s.frequency = (float)a.scalars[2];
+    s.temperature = (float)a.scalars[3];
+    if (const Tensor *h = given(a.history)) {
+        TORCH_CHECK(h->dim() == 2 && h->size(0) == B, fn, ": history must be [B, L]");
+        TORCH_CHECK(h->size(1) <= (1 << 24), fn, ": a history of ", h->size(1), " ids (at most 2^24)");
+        s.history = i64_rows(*h, fn), s.ld_history = h->stride(0), s.L = (int)h->size(1);
+        if (const Tensor *n = given(a.history_len)) {
+            s.len_per_row = per_row(*n, B, T, dims, fn, "history_len"), s.history_len = i32(*n, "history_len");
+        }
+        if (s.L == 0) s.history = nullptr, s.history_len = nullptr;
+    } else {
+        TORCH_CHECK(!given(a.history_len), fn, ": history_len without a history");
+    }
+    if (const Tensor *b = given(a.bias)) {
+        TORCH_CHECK((b->dim() == 1 || (b->dim() == 2 && b->size(0) == B)) && b->size(-1) == V, fn, ": bias must be [V] or [B, V]");
+        TORCH_CHECK(V == 1 || b->stride(-1) == 1, fn, ": bias needs contiguous rows");
+        s.bias = f32(*b, "bias"), s.ld_bias = b->dim() == 2 ? b->stride(0) : 0;
+    }
+    if (const Tensor *m = given(a.allowed)) {
+        TORCH_CHECK(m->is_cuda() && m->scalar_type() == at::kInt && m->dim() == 2 && m->size(0) >= 1 && m->size(1) == (V + 31) / 32 &&
+                        (m->size(1) == 1 || m->stride(1) == 1) && m->size(0) < (1ll << 31), fn,
+                    ": allowed must be int32 GPU words [states, ceil(V / 32)] with contiguous rows (ops.pack_allowed)");
+        s.allowed = m->const_data_ptr<int32_t>(), s.ld_allowed = m->size(0) > 1 ? m->stride(0) : m->size(1), s.S = (int)m->size(0);
+        if (const Tensor *w = given(a.state)) {
+            s.state_per_row = per_row(*w, B, T, dims, fn, "state"), s.state = i32(*w, "state");
+        } else {
+            TORCH_CHECK(s.S == 1 || s.S == B, fn, ": without states the mask table has one row, or one for each sequence");
+        }
+    } else {
+        TORCH_CHECK(!given(a.state), fn, ": states without a mask table");
+    }
+    return s;
+}
+#define PSVAE_SHAPING_PARAMS                                                                                             \
+    const Tensor &logits, const OptTensor &history, const OptTensor &history_len, const OptTensor &repetition,           \
+        const OptTensor &presence, const OptTensor &frequency, const OptTensor &temperature, at::ArrayRef<double> scalars, \
+        const OptTensor &bias, const OptTensor &allowed, const OptTensor &state
+#define PSVAE_SHAPING_ARGS {logits, history, history_len, repetition, presence, frequency, temperature, bias, allowed, state, scalars}
+#define PSVAE_SHAPING_TENSORS \
+    p(logits), p(history), p(history_len), p(repetition), p(presence), p(frequency), p(temperature), p(bias), p(allowed), p(state)
+#define PSVAE_SHAPING_SCHEMA                                                                                          \
+    "Tensor logits, Tensor? history, Tensor? history_len, Tensor? repetition, Tensor? presence, Tensor? frequency, " \
+    "Tensor? temperature, float[] scalars, Tensor? bias, Tensor? allowed, Tensor? state"
+
+// Scratch of one call: a tensor of its own from the allocator (stream-ordered, and inside a captured graph's own pool), so
+// that no two graphs or streams ever meet in it.
+Tensor scratch(size_t nbytes, const Tensor &like) { return at::empty({(int64_t)nbytes}, like.options().dtype(at::kByte)); }
+
+Tensor shape_logits(PSVAE_SHAPING_PARAMS) {
+    PSVAE_ON_DEVICE("psvae::shape_logits", PSVAE_SHAPING_TENSORS);
+    const char *fn = "psvae_shape_logits_fwd";
+    const psvae_shaping s = shaping_of(PSVAE_SHAPING_ARGS, fn);
+    Tensor out = at::empty(logits.sizes(), logits.options());
+    check(psvae_shape_logits_fwd(&s, out.data_ptr(), s.V, cur_stream(logits)), fn);
+    return out;
+}
+
+Tensor shape_logits_backward(const Tensor &g, PSVAE_SHAPING_PARAMS) {
+    PSVAE_ON_DEVICE("psvae::shape_logits_backward", p(g), PSVAE_SHAPING_TENSORS);
+    const char *fn = "psvae_shape_logits_bwd";
+    const psvae_shaping s = shaping_of(PSVAE_SHAPING_ARGS, fn);
+    TORCH_CHECK(g.sizes() == logits.sizes() && g.scalar_type() == logits.scalar_type(), fn, ": the gradient has the logits' shape and type");
+    const Tensor gc = s.V == 1 || g.stride(-1) == 1 ? g : g.contiguous();
+    Tensor out = at::empty(logits.sizes(), logits.options());
+    check(psvae_shape_logits_bwd(&s, gc.const_data_ptr(), gc.stride(0), gc.dim() == 3 ? gc.stride(1) : 0, out.data_ptr(), s.V,
+                                 cur_stream(logits)), fn);
+    return out;
+}
+
+const int64_t *row_tokens(const Tensor &tokens, const Tensor &logits, const char *fn) {
+    TORCH_CHECK(tokens.scalar_type() == at::kLong && tokens.is_contiguous() && tokens.sizes() == logits.sizes().slice(0, logits.dim() - 1), fn,
+                ": tokens must be contiguous int64, one for each row of the logits");
+    return tokens.const_data_ptr<int64_t>();
+}
+
+std::tuple<Tensor, Tensor> shaped_log_prob(const Tensor &tokens, PSVAE_SHAPING_PARAMS) {
+    PSVAE_ON_DEVICE("psvae::shaped_log_prob", p(tokens), PSVAE_SHAPING_TENSORS);
+    const char *fn = "psvae_shaped_log_prob_fwd";
+    const psvae_shaping s = shaping_of(PSVAE_SHAPING_ARGS, fn);
+    const int64_t *tok = row_tokens(tokens, logits, fn);
+    Tensor lp = at::empty(tokens.sizes(), logits.options().dtype(at::kFloat));
+    Tensor stats = at::empty({(int64_t)s.B * s.T, 2}, lp.options());
+    const size_t nbytes = psvae_shaped_log_prob_workspace_bytes(&s);
+    Tensor hold;
+    if (nbytes) hold = scratch(nbytes, logits);
+    check(psvae_shaped_log_prob_fwd(&s, tok, lp.data_ptr<float>(), stats.data_ptr<float>(), nbytes ? hold.data_ptr() : nullptr, nbytes,
+                                    cur_stream(logits)), fn);
+    return {lp, stats};
+}
+
+Tensor shaped_log_prob_backward(const Tensor &g, const Tensor &stats, const Tensor &tokens, PSVAE_SHAPING_PARAMS) {
+    PSVAE_ON_DEVICE("psvae::shaped_log_prob_backward", p(g), p(stats), p(tokens), PSVAE_SHAPING_TENSORS);
+    const char *fn = "psvae_shaped_log_prob_bwd";
+    const psvae_shaping s = shaping_of(PSVAE_SHAPING_ARGS, fn);
+    const int64_t *tok = row_tokens(tokens, logits, fn);
+    const int64_t rows = (int64_t)s.B * s.T;
+    TORCH_CHECK(g.scalar_type() == at::kFloat && g.sizes() == tokens.sizes() && stats.scalar_type() == at::kFloat && stats.is_contiguous() &&
+                    stats.dim() == 2 && stats.size(0) == rows && stats.size(1) == 2, fn, ": gradient [rows] and stats [rows, 2], float32");
+    const Tensor gc = g.contiguous();
+    Tensor out = at::empty(logits.sizes(), logits.options());
+    check(psvae_shaped_log_prob_bwd(&s, tok, stats.const_data_ptr<float>(), gc.const_data_ptr<float>(), out.data_ptr(), s.V, cur_stream(logits)), fn);
+    return out;
+}
+
+std::tuple<Tensor, Tensor> shaped_draw(const Tensor &uniforms, int64_t empty_token, PSVAE_SHAPING_PARAMS) {
+    PSVAE_ON_DEVICE("psvae::shaped_draw", p(uniforms), PSVAE_SHAPING_TENSORS);
+    const char *fn = "psvae_shaped_draw";
+    TORCH_CHECK(logits.dim() == 2, fn, ": logits must be [B, V]: one token per sequence is drawn");
+    const psvae_shaping s = shaping_of(PSVAE_SHAPING_ARGS, fn);
+    TORCH_CHECK(uniforms.dim() == 1 && uniforms.size(0) == logits.size(0), fn, ": uniforms must be [B]");
+    Tensor tokens = at::empty({logits.size(0)}, logits.options().dtype(at::kLong));
+    Tensor lp = at::empty({logits.size(0)}, logits.options().dtype(at::kFloat));
+    const size_t nbytes = psvae_shaped_draw_workspace_bytes(&s);
+    Tensor hold;
+    if (nbytes) hold = scratch(nbytes, logits);
+    check(psvae_shaped_draw(&s, f32(uniforms, "uniforms"), uniforms.size(0) > 1 ? uniforms.stride(0) : 1, empty_token,
+                            tokens.data_ptr<int64_t>(), lp.data_ptr<float>(), nbytes ? hold.data_ptr() : nullptr, nbytes, cur_stream(logits)), fn);
+    return {tokens, lp};
+}
+
+// ---- norm and clipping over a list of tensors
+struct TensorList {
+    std::vector<const void *> ptr;
+    std::vector<int64_t> numel;
+    std::vector<int32_t> types;
+};
+TensorList list_of(at::TensorList ts, c10::Device device, const char *fn) {
+    TensorList l;
+    l.ptr.reserve(ts.size()), l.numel.reserve(ts.size()), l.types.reserve(ts.size());
+    for (const Tensor &t : ts) {
+        TORCH_CHECK(t.is_cuda(), fn, ": psvae operators need GPU tensors (there is no CPU fallback)");
+        TORCH_CHECK(t.device() == device, fn, ": tensors on different devices (", device, " and ", t.device(), ")");
+        TORCH_CHECK(t.layout() == at::kStrided && t.is_non_overlapping_and_dense(), fn,
+                    ": a gradient must be dense, each of its elements in a place of its own");
+        l.ptr.push_back(t.const_data_ptr()), l.numel.push_back(t.numel()), l.types.push_back(elem_type(t, fn));
+    }
+    return l;
+}
+
+Tensor grad_norm(at::TensorList grads) {
+    const char *fn = "psvae_grad_norm";
+    TORCH_CHECK(!grads.empty(), fn, ": no tensors");
+    c10::DeviceGuard guard(same_device(fn, {&grads[0]}));
+    const TensorList l = list_of(grads, grads[0].device(), fn);
+    const int n = (int)grads.size();
+    Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat).memory_format(std::nullopt));
+    const size_t nbytes = psvae_grad_norm_workspace_bytes(n, l.numel.data());
+    Tensor hold = scratch(nbytes, norm);
+    check(psvae_grad_norm(n, l.ptr.data(), l.numel.data(), l.types.data(), norm.data_ptr<float>(), hold.data_ptr(), nbytes, cur_stream(norm)), fn);
+    return norm;
+}
+
+Tensor clip_grads(at::TensorList grads, double max_norm, at::TensorList out) {
+    const char *fn = "psvae_clip_grads";
+    TORCH_CHECK(!grads.empty() && out.size() == grads.size(), fn, ": one output for each of at least one gradient");
+    c10::DeviceGuard guard(same_device(fn, {&grads[0]}));
+    const TensorList l = list_of(grads, grads[0].device(), fn), o = list_of(out, grads[0].device(), fn);
+    const int n = (int)grads.size();
+    for (int i = 0; i < n; ++i)
+        TORCH_CHECK(out[i].numel() == grads[i].numel() &&
+                        (out[i].is_same(grads[i]) || (grads[i].is_contiguous() && out[i].is_contiguous()) ||
+                         (out[i].sizes() == grads[i].sizes() && out[i].strides() == grads[i].strides())), fn,
+                    ": output ", i, " must have its gradient's number of elements, in the same order in memory");
+    Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat).memory_format(std::nullopt));
+    const size_t nbytes = psvae_grad_norm_workspace_bytes(n, l.numel.data());
+    Tensor hold = scratch(nbytes, norm);
+    std::vector<void *> dst(n);
+    for (int i = 0; i < n; ++i) dst[i] = const_cast<void *>(o.ptr[i]);
+    check(psvae_clip_grads(n, l.ptr.data(), l.numel.data(), l.types.data(), dst.data(), o.types.data(), (float)max_norm,
+                           norm.data_ptr<float>(), hold.data_ptr(), nbytes, cur_stream(norm)), fn);
+    for (const Tensor &t : out)
+        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();   // (written through its pointer)
+    return norm;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(psvae, m) {
@@ -596,4 +822,11 @@ TORCH_LIBRARY(psvae, m) {
           &gru_seq_fwd);
     m.def("gru_seq_bwd(Tensor gates, Tensor ghn, Tensor hall, Tensor g_out, Tensor w_hh_t, Tensor(a!) dgi, Tensor(b!) dgh, "
           "Tensor(c!) dh0) -> ()", &gru_seq_bwd);
+    m.def("shape_logits(" PSVAE_SHAPING_SCHEMA ") -> Tensor", &shape_logits);
+    m.def("shape_logits_backward(Tensor g, " PSVAE_SHAPING_SCHEMA ") -> Tensor", &shape_logits_backward);
+    m.def("shaped_log_prob(Tensor tokens, " PSVAE_SHAPING_SCHEMA ") -> (Tensor, Tensor)", &shaped_log_prob);
+    m.def("shaped_log_prob_backward(Tensor g, Tensor stats, Tensor tokens, " PSVAE_SHAPING_SCHEMA ") -> Tensor", &shaped_log_prob_backward);
+    m.def("shaped_draw(Tensor uniforms, int empty_token, " PSVAE_SHAPING_SCHEMA ") -> (Tensor, Tensor)", &shaped_draw);
+    m.def("grad_norm(Tensor[] grads) -> Tensor", &grad_norm);
+    m.def("clip_grads(Tensor[] grads, float max_norm, Tensor(a!)[] out) -> Tensor", &clip_grads);
 }

@@ -96,6 +96,16 @@ _SIGNATURES = {
     'psvae_pair_enumerate_fill': (_c_int, [_c_int, _c_int, _p, _p, _p, _p, _p, _p, _p, _p, _p]),
     'psvae_piece_draw': (_c_int, [_c_int, _c_int, _p, _c_i64, _c_f32, _p, _c_i64, _c_int, _c_int, _c_int, _p, _c_int, _c_int,
                                   _p, _p, _p, _p, _c_i64, _p, _p]),
+    'psvae_shape_logits_fwd': (_c_int, [_p, _p, _c_i64, _p]),
+    'psvae_shape_logits_bwd': (_c_int, [_p, _p, _c_i64, _c_i64, _p, _c_i64, _p]),
+    'psvae_shaped_log_prob_workspace_bytes': (_c_size, [_p]),
+    'psvae_shaped_log_prob_fwd': (_c_int, [_p, _p, _p, _p, _p, _c_size, _p]),
+    'psvae_shaped_log_prob_bwd': (_c_int, [_p, _p, _p, _p, _p, _c_i64, _p]),
+    'psvae_shaped_draw_workspace_bytes': (_c_size, [_p]),
+    'psvae_shaped_draw': (_c_int, [_p, _p, _c_i64, _c_i64, _p, _p, _p, _c_size, _p]),
+    'psvae_grad_norm_workspace_bytes': (_c_size, [_c_int, _p]),
+    'psvae_grad_norm': (_c_int, [_c_int, _p, _p, _p, _p, _p, _c_size, _p]),
+    'psvae_clip_grads': (_c_int, [_c_int, _p, _p, _p, _p, _p, _c_f32, _p, _p, _c_size, _p]),
     'psvae_embed_trans_fwd': (_c_int, [_c_int, _c_int, _p, _p, _p, _c_int, _c_int, _c_int, _p, _p, _c_int, _p]),
     'psvae_clip_adam_workspace_bytes': (_c_size, [_c_ll]),
     'psvae_clip_adam_step': (_c_int, [_c_ll, _p, _p, _p, _p, _c_f32, _c_f32] + [_c_f64] * 5 + [_c_int, _c_int, _p, _p, _c_size, _p]),
@@ -103,6 +113,19 @@ _SIGNATURES = {
     'psvae_assemble_links_workspace_bytes': (_c_size, [_c_int]),
     'psvae_assemble_links': (_c_int, [_c_int, _c_int] + [_p] * 12 + [_c_int, _c_int] + [_p] * 5 + [_c_size, _p]),
 }
+
+F32, BF16, F16 = 0, 1, 2   # PSVAE_F32 / PSVAE_BF16 / PSVAE_F16
+
+
+class Shaping(ctypes.Structure):
+    """psvae_shaping: what a call over shaped logits works on (callers of the C ABI; torch.ops.psvae fills it from tensors)."""
+    _fields_ = [('B', _c_int), ('T', _c_int), ('V', _c_int), ('dtype', _c_int), ('logits', _p), ('ld_b', _c_i64), ('ld_t', _c_i64),
+                ('history', _p), ('ld_history', _c_i64), ('L', _c_int), ('history_len', _p), ('len_per_row', _c_int),
+                ('repetition_rows', _p), ('presence_rows', _p), ('frequency_rows', _p), ('temperature_rows', _p),
+                ('repetition', _c_f32), ('presence', _c_f32), ('frequency', _c_f32), ('temperature', _c_f32),
+                ('bias', _p), ('ld_bias', _c_i64), ('allowed', _p), ('ld_allowed', _c_i64), ('S', _c_int), ('state', _p),
+                ('state_per_row', _c_int)]
+
 
 _lib = None
 
@@ -685,6 +708,45 @@ def piece_draw(logits, temperature, uniforms_col, pad, end, first_step, piece_at
                                   ptr(active, torch.uint8), ptr(atoms, torch.int32), ptr(length, torch.int32),
                                   ptr(out_col, torch.int64), out_col.stride(0) if B > 1 else 1, ptr(cur, torch.int64),
                                   _stream()), 'psvae_piece_draw')
+
+
+def shape_logits(*shaping):
+    """psvae_shape_logits_fwd; `shaping`: logits, history, history_len, repetition, presence, frequency, temperature
+    (tensors or None), the four scalars that stand in for them, bias, allowed, state."""
+    _count()
+    return ops().shape_logits(*shaping)
+
+
+def shape_logits_backward(g, *shaping):
+    _count()
+    return ops().shape_logits_backward(g, *shaping)
+
+
+def shaped_log_prob(tokens, *shaping):
+    """(log-probabilities, stats) of psvae_shaped_log_prob_fwd."""
+    _count()
+    return ops().shaped_log_prob(tokens, *shaping)
+
+
+def shaped_log_prob_backward(g, stats, tokens, *shaping):
+    _count()
+    return ops().shaped_log_prob_backward(g, stats, tokens, *shaping)
+
+
+def shaped_draw(uniforms, empty_token, *shaping):
+    """(tokens, log-probabilities) of psvae_shaped_draw."""
+    _count()
+    return ops().shaped_draw(uniforms, empty_token, *shaping)
+
+
+def grad_norm(grads):
+    _count()
+    return ops().grad_norm(grads)
+
+
+def clip_grads(grads, max_norm, out):
+    _count()
+    return ops().clip_grads(grads, max_norm, out)
 
 
 def link_infer(logits, add_edge_th, none_bond, conf, etype, keep):

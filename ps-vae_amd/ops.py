@@ -1007,3 +1007,112 @@ def linear_relu_classes(x, weight, bias, cls_weight, cls_bias):
     hip.gemm_relu_classes(x, weight.detach(), None if bias is None else bias.detach(), w4.contiguous(), partials)
     logits = partials.sum(dim=1)[:, :C]
     return logits + cls_bias.detach() if cls_bias is not None else logits
+
+
+# ------------------------------------------------------------------------ shaped logits
+def pack_allowed(allowed):
+    """Mask table of a grammar as the operators below read it: bool [S, V] (row s: the tokens that state s allows) ->
+    int32 [S, ceil(V / 32)], bit i % 32 of word i / 32.  Made once; the states change from step to step."""
+    if allowed.dim() != 2 or allowed.dtype != torch.bool:
+        raise ValueError('pack_allowed: need a bool table [states, vocabulary]')
+    S, V = allowed.shape
+    W = (V + 31) // 32
+    bits = torch.zeros(S, W * 32, dtype=torch.int64, device=allowed.device)
+    bits[:, :V] = allowed
+    place = torch.ones(32, dtype=torch.int64, device=allowed.device) << torch.arange(32, device=allowed.device)
+    words = (bits.view(S, W, 32) * place).sum(-1)
+    return torch.where(words >= 1 << 31, words - (1 << 32), words).to(torch.int32)
+
+
+_NEUTRAL = (1.0, 0.0, 0.0, 1.0)   # repetition, presence, frequency, temperature that change nothing
+
+
+def _shaping(logits, history, history_len, repetition, presence, frequency, bias, allowed, state, temperature):
+    """The operators' arguments behind the logits, in the order of torch.ops.psvae.shape_logits: a penalty or temperature is
+    either a tensor with one value per sequence or one number for all."""
+    tensors, numbers = [], []
+    for v, neutral in zip((repetition, presence, frequency, temperature), _NEUTRAL):
+        is_tensor = torch.is_tensor(v)
+        tensors.append(v if is_tensor else None)
+        numbers.append(neutral if v is None or is_tensor else float(v))
+    if history is None and (repetition is not None or presence is not None or frequency is not None):
+        raise ValueError('penalties need a history')
+    for t in (bias, *tensors):
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise ValueError('penalties, bias and temperature are data: none of them gets a gradient')
+    return (history, history_len, *tensors, numbers, bias, allowed, state)
+
+
+class _ShapeLogits(Function):
+    @staticmethod
+    def forward(ctx, logits, *shaping):
+        ctx.save_for_backward(logits, *(t for t in shaping if torch.is_tensor(t)))
+        ctx.shaping = [None if torch.is_tensor(t) else (t,) for t in shaping]   # (None: a saved tensor's place)
+        return hip.shape_logits(logits, *shaping)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        saved = iter(ctx.saved_tensors)
+        logits = next(saved)
+        return (hip.shape_logits_backward(g, logits, *(next(saved) if t is None else t[0] for t in ctx.shaping)),
+                *[None] * len(ctx.shaping))
+
+
+class _ShapedLogProb(Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, *shaping):
+        lp, stats = hip.shaped_log_prob(tokens, logits, *shaping)
+        ctx.save_for_backward(logits, tokens, stats, *(t for t in shaping if torch.is_tensor(t)))
+        ctx.shaping = [None if torch.is_tensor(t) else (t,) for t in shaping]
+        return lp
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        saved = iter(ctx.saved_tensors)
+        logits, tokens, stats = next(saved), next(saved), next(saved)
+        return (hip.shaped_log_prob_backward(g, stats, tokens, logits, *(next(saved) if t is None else t[0] for t in ctx.shaping)),
+                *[None] * (1 + len(ctx.shaping)))
+
+
+def shape_logits(logits, *, history=None, history_len=None, repetition=None, presence=None, frequency=None, bias=None,
+                 allowed=None, state=None, temperature=None):
+    """Logits [B, V] or [B, T, V] (float32, bfloat16, float16; contiguous rows) of a language model, shaped for the choice of the
+    next token; the result has their shape and type.  Row (b, t), with c_i the number of times id i occurs among the first
+    history_len ids of history[b]:
+
+        a_i = l_i;   c_i > 0:  a_i = (l_i / repetition if l_i > 0 else l_i * repetition) - frequency * c_i - presence
+        y_i = (a_i + bias_i) / temperature   where the row's mask allows i, else -inf
+
+    history int64 [B, L] (ids outside the vocabulary count for nothing: padding may be negative); history_len int32 [B] or
+    [B, T] (None: L).  repetition, presence, frequency, temperature: a number or float32 [B].  bias float32 [V] or [B, V].
+    allowed: a table of masks (pack_allowed); state int32 [B] or [B, T]: the table's row for each row of logits - negative: nothing is
+    forbidden, past the table: everything is; None: the table has one row for all, or one per sequence.
+
+    Differentiable in the logits (once); masked places get no gradient and what they hold is never looked at."""
+    shaping = _shaping(logits, history, history_len, repetition, presence, frequency, bias, allowed, state, temperature)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _ShapeLogits.apply(logits, *shaping)
+    return hip.shape_logits(logits, *shaping)
+
+
+def shaped_log_prob(logits, tokens, *, history=None, history_len=None, repetition=None, presence=None, frequency=None, bias=None,
+                    allowed=None, state=None, temperature=None):
+    """log softmax(y)[token] in float32, y as shape_logits shapes it (same arguments; never written out): tokens int64 [B] or
+    [B, T], one for each row.  A token outside the vocabulary: 0 and no gradient (padding).  A token that the mask forbids, or a row
+    that allows none: -inf (the latter without gradient).  Differentiable in the logits (once)."""
+    shaping = _shaping(logits, history, history_len, repetition, presence, frequency, bias, allowed, state, temperature)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _ShapedLogProb.apply(logits, tokens, *shaping)
+    return hip.shaped_log_prob(tokens, logits, *shaping)[0]
+
+
+def shaped_draw(logits, uniforms, *, history=None, history_len=None, repetition=None, presence=None, frequency=None, bias=None,
+                allowed=None, state=None, temperature=None, empty_token=-1):
+    """One token per sequence from softmax(y) of logits [B, V], y as shape_logits shapes it: the first index whose running sum of
+    probabilities exceeds uniforms[b] (float32 [B] in [0, 1)) times their total.  Returns (tokens int64 [B], log-probabilities
+    float32 [B]).  A row that allows no token gives empty_token and -inf, one with NaN or +inf among its allowed values empty_token
+    and NaN."""
+    shaping = _shaping(logits, history, history_len, repetition, presence, frequency, bias, allowed, state, temperature)
+    return hip.shaped_draw(uniforms, empty_token, logits, *shaping)

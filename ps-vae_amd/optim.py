@@ -95,3 +95,30 @@ class FlatAdam(torch.optim.Optimizer):
             self.exp_avg_sq.copy_(state['exp_avg_sq'])
         for g, saved in zip(self.param_groups, state['param_groups']):
             g.update({k: v for k, v in saved.items() if k != 'params'})
+
+
+@torch.no_grad()
+def grad_norm(grads):
+    """2-norm (float32 scalar on the GPU) over a list of gradient tensors, each dense, of float32, bfloat16 or float16, on one
+    device: squares and sums in 64 bits, the same bits for the same sizes and values.  Nothing is copied together; capturable."""
+    return hip.grad_norm(list(grads))
+
+
+@torch.no_grad()
+def clip_grads(grads, max_norm, out=None):
+    """Scales a list of gradient tensors (as grad_norm takes) by min(1, max_norm / (norm + 1e-6)), norm their common 2-norm, and
+    returns the norm.  In place; or into `out`, one tensor per gradient with as many elements - the slices of a flat float32
+    buffer, say, for gradients in bfloat16.  A norm that is not a number makes every gradient NaN, as torch's clip_grad_norm_ does."""
+    grads = list(grads)
+    return hip.clip_grads(grads, float(max_norm), grads if out is None else list(out))
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm):
+    """torch.nn.utils.clip_grad_norm_(parameters, max_norm) (norm_type 2) on the GPU for parameters of any mix of float types: two
+    kernel launches up to 120 gradients, whatever their sizes."""
+    parameters = [parameters] if torch.is_tensor(parameters) else list(parameters)
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not grads:
+        return torch.zeros((), dtype=torch.float32, device=parameters[0].device if parameters else None)
+    return clip_grads(grads, max_norm)
