@@ -122,26 +122,78 @@ template <typename T> __device__ __forceinline__ void store_pack(T *p, const Pac
     }
 }
 
-// The shaped value in type C (float, double) and, for the gradient, its slope.
+// ---- bits.  Bit j of `bits` as a word of ones or zeros: one bit-field extract, and a masked value is then one bit-select
+// (a compare and a conditional move per value would be three).
+__device__ __forceinline__ int bit_word(uint32_t bits, int j) { return (int)(bits << (31 - j)) >> 31; }
+__device__ __forceinline__ float select(int word, float yes, float no) {
+    return __int_as_float((word & __float_as_int(yes)) | (~word & __float_as_int(no)));
+}
+__device__ __forceinline__ double select(int word, double yes, double no) {
+    const long long w = word;
+    return __longlong_as_double((w & __double_as_longlong(yes)) | (~w & __double_as_longlong(no)));
+}
+
+// ---- sums and maxima over the wave in the vector unit's own lane permutes: within rows of 16 lanes, then from row to row.  A lane
+// without a source takes `none`.
+template <int CTRL, int ROWS> __device__ __forceinline__ float lane_move(float none, float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(none), __float_as_int(v), CTRL, ROWS, 0xf, false));
+}
+template <int CTRL, int ROWS> __device__ __forceinline__ double lane_move(double none, double v) {
+    const long long n = __double_as_longlong(none), x = __double_as_longlong(v);
+    const int lo = __builtin_amdgcn_update_dpp((int)n, (int)x, CTRL, ROWS, 0xf, false);
+    const int hi = __builtin_amdgcn_update_dpp((int)(n >> 32), (int)(x >> 32), CTRL, ROWS, 0xf, false);
+    return __longlong_as_double((long long)(((unsigned long long)(unsigned)hi << 32) | (unsigned)lo));
+}
+constexpr int ROW_SHR1 = 0x111, ROW_SHR2 = 0x112, ROW_SHR4 = 0x114, ROW_SHR8 = 0x118, BCAST15 = 0x142, BCAST31 = 0x143;
+
+__device__ __forceinline__ float from_lane(float v, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane)); }
+__device__ __forceinline__ double from_lane(double v, int lane) {
+    const long long x = __double_as_longlong(v);
+    const int lo = __builtin_amdgcn_readlane((int)x, lane), hi = __builtin_amdgcn_readlane((int)(x >> 32), lane);
+    return __longlong_as_double((long long)(((unsigned long long)(unsigned)hi << 32) | (unsigned)lo));
+}
+template <typename C> __device__ __forceinline__ C wave_scan(C v) {   // inclusive, in lane order
+    v += lane_move<ROW_SHR1, 0xf>((C)0, v);
+    v += lane_move<ROW_SHR2, 0xf>((C)0, v);
+    v += lane_move<ROW_SHR4, 0xf>((C)0, v);
+    v += lane_move<ROW_SHR8, 0xf>((C)0, v);
+    v += lane_move<BCAST15, 0xa>((C)0, v);
+    v += lane_move<BCAST31, 0xc>((C)0, v);
+    return v;
+}
+template <typename C> __device__ __forceinline__ C wave_sum(C v) { return from_lane(wave_scan(v), 63); }
+__device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ double larger(double a, double b) { return fmax(a, b); }
+template <typename C> __device__ __forceinline__ C wave_max(C v) {
+    const C none = (C)NEG;
+    v = larger(v, lane_move<ROW_SHR1, 0xf>(none, v));
+    v = larger(v, lane_move<ROW_SHR2, 0xf>(none, v));
+    v = larger(v, lane_move<ROW_SHR4, 0xf>(none, v));
+    v = larger(v, lane_move<ROW_SHR8, 0xf>(none, v));
+    v = larger(v, lane_move<BCAST15, 0xa>(none, v));
+    v = larger(v, lane_move<BCAST31, 0xc>(none, v));
+    return from_lane(v, 63);
+}
+
+// The penalties and the last factor of a row in type C (float; double for draws).  `unit` scales the result: 1, or log2 e where it goes
+// into a power of two.
 template <typename C> struct Rule {
-    C rep, pres, freq, inv_temp;
-    template <typename T> __device__ Rule(const Row<T> &w)
-        : rep((C)w.rep), pres((C)w.pres), freq((C)w.freq), inv_temp((C)1 / (C)w.temp) {}
-    __device__ __forceinline__ C value(C x, int c, C bias) const {
-        if (c > 0) x = (x > (C)0 ? x / rep : x * rep) - freq * (C)c - pres;
-        return (x + bias) * inv_temp;
-    }
-    __device__ __forceinline__ C slope(C x, int c) const { return c > 0 ? (x > (C)0 ? inv_temp / rep : inv_temp * rep) : inv_temp; }
+    C rep, inv_rep, pres, freq, scale;
+    template <typename T> __device__ Rule(const Row<T> &w, C unit)
+        : rep((C)w.rep), inv_rep((C)1 / (C)w.rep), pres((C)w.pres), freq((C)w.freq), scale(unit / (C)w.temp) {}
+    __device__ __forceinline__ C factor(C x) const { return x > (C)0 ? inv_rep : rep; }   // what a seen token's logit is multiplied by
+    __device__ __forceinline__ C penalised(C x, int c) const { return c > 0 ? x * factor(x) - (freq * (C)c + pres) : x; }
 };
 
-// VEC bits of the mask for the elements i .. i + VEC - 1 (i a multiple of VEC)
-template <int VEC> __device__ __forceinline__ uint32_t mask_bits(const uint32_t *mask, int i) {
-    return mask ? (mask[i >> 5] >> (i & 31)) : 0xffffffffu;
+// y in units of 1 / scale, rounded by itself.  Equal values have to stay equal: fused with the subtraction of the row's maximum that follows, the
+// product would keep its unrounded rest, which for values near the type's lowest is far from 0.
+template <typename C> __device__ __forceinline__ C scaled(C y, C scale) {
+#pragma clang fp contract(off)
+    return y * scale;
 }
+
+// The bias of VEC elements, zeros past the row's end.
 template <int VEC> __device__ __forceinline__ void load_bias(const float *bias, int left, float (&b)[VEC]) {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) b[j] = 0.f;
-    if (!bias) return;
     if (left >= VEC) {
 #pragma unroll
         for (int q = 0; q < VEC / 4; ++q) {
@@ -151,8 +203,7 @@ template <int VEC> __device__ __forceinline__ void load_bias(const float *bias, 
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j)
-            if (j < left) b[j] = bias[j];
+        for (int j = 0; j < VEC; ++j) b[j] = j < left ? bias[j] : 0.f;
     }
 }
 
@@ -162,11 +213,11 @@ template <typename T, int K, int ROWS> struct Place {
     int r, unit, tid, lane, wave;    // row; unit of the row; thread, lane and wave inside the row's group
     bool live;
     __device__ Place(const Args &a, int block) {
-        tid = threadIdx.x & (THREADS - 1), lane = threadIdx.x & 63, wave = tid >> 6;
+        tid = threadIdx.x & (THREADS - 1), lane = threadIdx.x & 63, wave = ROWS == 1 ? __builtin_amdgcn_readfirstlane(tid >> 6) : 0;
         if (ROWS == 1) {
             r = a.units == 1 ? block : (int)((unsigned)block / (unsigned)a.units), unit = block - r * a.units;
         } else {
-            r = block * ROWS + (int)threadIdx.x / THREADS, unit = 0;
+            r = block * ROWS + __builtin_amdgcn_readfirstlane((int)threadIdx.x / THREADS), unit = 0;
         }
         live = r < a.R;
         if (!live) r = a.R - 1;
@@ -175,7 +226,7 @@ template <typename T, int K, int ROWS> struct Place {
     __device__ __forceinline__ int at(int k) const { return ((wave * K + k) * 64 + lane) * VEC; }   // inside the unit
 };
 
-// Loads a thread's logits, counts the unit, and hands out (element, left, count, bits, bias) per VEC.
+// Loads a thread's logits, counts the unit, and hands out what belongs to pack k of it.
 template <typename T, int K, int ROWS, bool HIST> struct Unit {
     using P = Place<T, K, ROWS>;
     static constexpr int VEC = P::VEC;
@@ -183,24 +234,63 @@ template <typename T, int K, int ROWS, bool HIST> struct Unit {
     Row<T> w;
     Pack<T> x[K];
     int *cnt;
-    int V;
-    __device__ Unit(const Args &a, int block, int *lds, bool want_logits) : p(a, block), w(row_of<T>(a, p.r)), V(a.V) {
+    int n;                           // elements of the unit that the row has
+    __device__ Unit(const Args &a, int block, int *lds, bool want_logits) : p(a, block), w(row_of<T>(a, p.r)) {
         const int base = p.base();
+        n = p.live ? (a.V - base < P::SPAN ? a.V - base : P::SPAN) : 0;
         if (want_logits) {
+            if (n == P::SPAN) {      // (no lane's load hangs on a test of its own)
 #pragma unroll
-            for (int k = 0; k < K; ++k) x[k] = load_pack(w.x + base + p.at(k), p.live ? V - base - p.at(k) : 0);
+                for (int k = 0; k < K; ++k) x[k] = *reinterpret_cast<const Pack<T> *>(w.x + base + p.at(k));
+            } else {
+#pragma unroll
+                for (int k = 0; k < K; ++k) x[k] = load_pack(w.x + base + p.at(k), n - p.at(k));
+            }
         }
         cnt = HIST ? lds + (ROWS == 1 ? 0 : (int)threadIdx.x / P::THREADS * P::SPAN) : nullptr;
-        if (HIST) {
-            const int n = V - base < P::SPAN ? V - base : P::SPAN;
-            count_unit(cnt, P::SPAN, w.hist, p.live ? w.len : 0, base, n, p.tid, P::THREADS);
-        }
+        if (HIST) count_unit(cnt, P::SPAN, w.hist, p.live ? w.len : 0, base, n, p.tid, P::THREADS);
     }
-    __device__ __forceinline__ int left(int k) const { return p.live ? V - p.base() - p.at(k) : 0; }
+    __device__ __forceinline__ int left(int k) const { return n - p.at(k); }
+    __device__ __forceinline__ int element(int k) const { return p.base() + p.at(k); }
+    // bit j: element j of the pack is in the row and allowed
     __device__ __forceinline__ uint32_t bits(int k) const {
-        return w.none || left(k) <= 0 ? 0u : mask_bits<VEC>(w.mask, p.base() + p.at(k));
+        const int l = left(k);
+        if (w.none || l <= 0) return 0u;
+        const int i = element(k);
+        const uint32_t b = w.mask ? w.mask[i >> 5] >> (i & 31) : 0xffffffffu;   // (i is a multiple of VEC: one word)
+        return l >= VEC ? b : b & ((1u << l) - 1u);
     }
-    __device__ __forceinline__ int count(int k, int j) const { return HIST ? cnt[p.at(k) + j] : 0; }
+    // the counts of the pack; whether any lane of the wave has one above 0
+    __device__ __forceinline__ bool counts(int k, int (&c)[VEC]) const {
+        int any = 0;
+#pragma unroll
+        for (int q = 0; q < VEC / 4; ++q) {
+            const int4 v = *reinterpret_cast<const int4 *>(cnt + p.at(k) + 4 * q);
+            c[4 * q] = v.x, c[4 * q + 1] = v.y, c[4 * q + 2] = v.z, c[4 * q + 3] = v.w;
+            any |= (v.x | v.y) | (v.z | v.w);
+        }
+        return __ballot(any != 0) != 0;
+    }
+    // y of the pack, before the mask
+    template <typename C> __device__ __forceinline__ void values(int k, const Rule<C> &rule, C (&y)[VEC]) const {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) y[j] = (C)(float)x[k].v[j];
+        if (HIST) {
+            int c[VEC];
+            if (counts(k, c)) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) y[j] = rule.penalised(y[j], c[j]);
+            }
+        }
+        if (w.bias) {
+            float b[VEC];
+            load_bias<VEC>(w.bias + element(k), left(k), b);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) y[j] += (C)b[j];
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) y[j] = scaled(y[j], rule.scale);
+    }
 };
 
 template <typename T, int K, int ROWS, bool HIST>
@@ -208,80 +298,61 @@ __global__ __launch_bounds__(NT) void shape_fwd_kernel(Args a, T *__restrict__ o
     using U = Unit<T, K, ROWS, HIST>;
     __shared__ __align__(16) int lds[HIST ? U::P::SPAN * ROWS : 4];
     U u(a, blockIdx.x, lds, true);
-    if (!u.p.live) return;
-    const Rule<float> rule(u.w);
+    const Rule<float> rule(u.w, 1.f);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const int left = u.left(k);
-        if (left <= 0) continue;
-        const int i = u.p.base() + u.p.at(k);
         const uint32_t bits = u.bits(k);
-        float b[U::VEC];
-        load_bias<U::VEC>(u.w.bias ? u.w.bias + i : nullptr, left, b);
+        float v[U::VEC];
+        u.values(k, rule, v);
         Pack<T> y;
 #pragma unroll
-        for (int j = 0; j < U::VEC; ++j) {
-            const float v = rule.value((float)u.x[k].v[j], u.count(k, j), b[j]);
-            y.v[j] = (T)((bits >> j) & 1u ? v : NEG);
-        }
-        store_pack(out + u.p.r * ld_out + i, y, left);
+        for (int j = 0; j < U::VEC; ++j) y.v[j] = (T)select(bit_word(bits, j), v[j], NEG);
+        store_pack(out + u.p.r * ld_out + u.element(k), y, u.left(k));
     }
 }
 
-// dl = g * slope; the logits are read only where a past token's sign decides the slope (x != null).
+// dl = g dy/dl; the logits are read only where the sign of a seen token's decides.
 template <typename T, int K, int ROWS, bool HIST>
 __global__ __launch_bounds__(NT) void shape_bwd_kernel(Args a, const T *__restrict__ g, long long ld_gb, long long ld_gt,
                                                        T *__restrict__ dx, long long ld_dx) {
     using U = Unit<T, K, ROWS, HIST>;
     __shared__ __align__(16) int lds[HIST ? U::P::SPAN * ROWS : 4];
     U u(a, blockIdx.x, lds, false);
-    if (!u.p.live) return;
-    const Rule<float> rule(u.w);
+    const Rule<float> rule(u.w, 1.f);
     const int b = a.T == 1 ? u.p.r : (int)((unsigned)u.p.r / (unsigned)a.T), t = u.p.r - b * a.T;
     const T *gr = g + b * ld_gb + t * ld_gt;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const int left = u.left(k);
-        if (left <= 0) continue;
-        const int i = u.p.base() + u.p.at(k);
         const uint32_t bits = u.bits(k);
-        const Pack<T> gv = load_pack(gr + i, left);
+        const int i = u.element(k);
+        const Pack<T> gv = load_pack(gr + i, u.left(k));
+        float v[U::VEC];
+#pragma unroll
+        for (int j = 0; j < U::VEC; ++j) v[j] = (float)gv.v[j] * rule.scale;
+        if (HIST) {
+            int c[U::VEC];
+            if (u.counts(k, c)) {
+#pragma unroll
+                for (int j = 0; j < U::VEC; ++j)
+                    if (c[j] > 0) v[j] *= rule.factor((float)u.w.x[i + j]);
+            }
+        }
         Pack<T> d;
 #pragma unroll
-        for (int j = 0; j < U::VEC; ++j) {
-            const int c = u.count(k, j);
-            float x = 0.f;
-            if (c > 0) x = (float)u.w.x[i + j];
-            d.v[j] = (T)((bits >> j) & 1u ? (float)gv.v[j] * rule.slope(x, c) : 0.f);
-        }
-        store_pack(dx + u.p.r * ld_dx + i, d, left);
+        for (int j = 0; j < U::VEC; ++j) d.v[j] = (T)select(bit_word(bits, j), v[j], 0.f);
+        store_pack(dx + u.p.r * ld_dx + i, d, u.left(k));
     }
-}
-
-__device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
-__device__ __forceinline__ double larger(double a, double b) { return fmax(a, b); }
-template <typename C> __device__ __forceinline__ C wave_max(C v) {
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) v = larger(v, __shfl_xor(v, d));
-    return v;
-}
-template <typename C> __device__ __forceinline__ C wave_sum(C v) {
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d);
-    return v;
-}
-template <typename C> __device__ __forceinline__ C wave_scan(C v, int lane) {   // inclusive, in lane order
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const C up = __shfl_up(v, d);
-        if (lane >= d) v += up;
-    }
-    return v;
 }
 
 __device__ __forceinline__ float log_prob_of(float y_tok, float m, float s) {
     return m == NEG && s == 0.f ? NEG : y_tok - m - logf(s);   // (nothing allowed: log 0)
 }
+
+// exp(y - m) as a power of two.  (The difference first: a row of the type's lowest values - masked by hand - has an m whose multiple of
+// log2 e overflows.)  A piece that allows nothing has m = -inf: 0 in its place.
+constexpr float LOG2E = 1.4426950408889634f;
+__device__ __forceinline__ float reference_of(float m) { return m == NEG ? 0.f : m; }
+__device__ __forceinline__ float exp_from(float y, float m) { return __builtin_amdgcn_exp2f((y - m) * LOG2E); }
 
 // Per wave: the maximum and the sum of exponentials of its piece; per row: the shaped value of its token.  ROWS > 1: the wave has the
 // whole row and finishes it.  Sums are 32-bit: 64 lanes of at most VEC * K terms each, then 6 levels, so the relative error stays below
@@ -294,30 +365,35 @@ __global__ __launch_bounds__(NT) void log_prob_fwd_kernel(Args a, const int64_t 
     __shared__ __align__(16) int lds[HIST ? U::P::SPAN * ROWS : 4];
     U u(a, blockIdx.x, lds, true);
     if (!u.p.live) return;
-    const Rule<float> rule(u.w);
+    const Rule<float> rule(u.w, 1.f);
     const long long tok = tokens[u.p.r];
     float y[K][U::VEC];
     float m = NEG, yt = 0.f;
     bool mine = false;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const int left = u.left(k), i = u.p.base() + u.p.at(k);
         const uint32_t bits = u.bits(k);
-        float b[U::VEC];
-        load_bias<U::VEC>(u.w.bias ? u.w.bias + i : nullptr, left, b);
+        u.values(k, rule, y[k]);
 #pragma unroll
         for (int j = 0; j < U::VEC; ++j) {
-            y[k][j] = j < left && ((bits >> j) & 1u) ? rule.value((float)u.x[k].v[j], u.count(k, j), b[j]) : NEG;
+            y[k][j] = select(bit_word(bits, j), y[k][j], NEG);
             m = fmaxf(m, y[k][j]);
-            if (j < left && i + j == tok) yt = y[k][j], mine = true;
+        }
+        const long long at = tok - u.element(k);
+        if (at >= 0 && at < U::VEC && at < u.left(k)) {
+            mine = true;
+#pragma unroll
+            for (int j = 0; j < U::VEC; ++j)
+                if (j == at) yt = y[k][j];
         }
     }
     m = wave_max(m);
+    const float from = reference_of(m);
     float s = 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int j = 0; j < U::VEC; ++j) s += y[k][j] == NEG ? 0.f : __expf(y[k][j] - m);
+        for (int j = 0; j < U::VEC; ++j) s += exp_from(y[k][j], from);
     s = wave_sum(s);
     if (ROWS == 1) {
         if (mine) target[u.p.r] = yt;
@@ -325,7 +401,7 @@ __global__ __launch_bounds__(NT) void log_prob_fwd_kernel(Args a, const int64_t 
         return;
     }
     const unsigned long long owner = __ballot(mine);
-    const float v = owner ? log_prob_of(__shfl(yt, __ffsll((long long)owner) - 1), m, s) : 0.f;
+    const float v = owner ? log_prob_of(from_lane(yt, __ffsll((long long)owner) - 1), m, s) : 0.f;
     if (u.p.lane == 0) lp[u.p.r] = v, stats[u.p.r] = make_float2(m, s);
 }
 
@@ -357,97 +433,129 @@ __global__ __launch_bounds__(NT) void log_prob_bwd_kernel(Args a, const int64_t 
     using U = Unit<T, K, ROWS, HIST>;
     __shared__ __align__(16) int lds[HIST ? U::P::SPAN * ROWS : 4];
     U u(a, blockIdx.x, lds, true);
-    if (!u.p.live) return;
-    const Rule<float> rule(u.w);
+    const Rule<float> rule(u.w, 1.f);
     const long long tok = tokens[u.p.r];
     const float2 st = stats[u.p.r];
     const bool zero = tok < 0 || tok >= a.V || (st.x == NEG && st.y == 0.f);   // a row without a token, or with none allowed
-    const float gr = g[u.p.r], inv = 1.f / st.y;
+    const float at_token = g[u.p.r] * rule.scale, others = -at_token / st.y, from = reference_of(st.x);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const int left = u.left(k);
-        if (left <= 0) continue;
-        const int i = u.p.base() + u.p.at(k);
         const uint32_t bits = zero ? 0u : u.bits(k);
-        float b[U::VEC];
-        load_bias<U::VEC>(u.w.bias ? u.w.bias + i : nullptr, left, b);
+        const int i = u.element(k);
+        float v[U::VEC];
+        u.values(k, rule, v);
+#pragma unroll
+        for (int j = 0; j < U::VEC; ++j) v[j] = others * exp_from(v[j], from);
+        const long long at = tok - i;
+        if (at >= 0 && at < U::VEC) {
+#pragma unroll
+            for (int j = 0; j < U::VEC; ++j)
+                if (j == at) v[j] += at_token;
+        }
+        if (HIST) {
+            int c[U::VEC];
+            if (u.counts(k, c)) {
+#pragma unroll
+                for (int j = 0; j < U::VEC; ++j)
+                    if (c[j] > 0) v[j] *= rule.factor((float)u.x[k].v[j]);
+            }
+        }
         Pack<T> d;
 #pragma unroll
-        for (int j = 0; j < U::VEC; ++j) {
-            const int c = u.count(k, j);
-            const float x = (float)u.x[k].v[j];
-            const float p = __expf(rule.value(x, c, b[j]) - st.x) * inv;
-            d.v[j] = (T)((bits >> j) & 1u ? gr * ((i + j == tok ? 1.f : 0.f) - p) * rule.slope(x, c) : 0.f);
-        }
-        store_pack(dx + u.p.r * ld_dx + i, d, left);
+        for (int j = 0; j < U::VEC; ++j) d.v[j] = (T)select(bit_word(bits, j), v[j], 0.f);
+        store_pack(dx + u.p.r * ld_dx + i, d, u.left(k));
     }
 }
 
 // ---- draw.  The pick is a decision: with a running sum in 32 bits, u * total falls on the wrong side of some boundary about once in
 // 1e3 .. 1e4 rows at V = 1e5 (V boundaries, each off by ~1e-8), and differently for every tiling.  So values, exponentials and sums are
-// 64-bit here: the pick is the one of the exact distribution but for ~1e-11 of the rows, whatever the tiling.
+// 64-bit here: the pick is the one of the exact distribution but for ~1e-9 of the rows, whatever the tiling.
 struct Piece {
-    double s, m;
+    double s, m;                     // sum of 2^(z - m), largest z;  z = y log2 e
 };
-constexpr double NEG64 = -__builtin_inf();
+constexpr double NEG64 = -__builtin_inf(), LOG2E64 = 1.4426950408889634;
 
-// e[k][j] = exp(y - m) of the thread's elements (0 where not allowed); returns m, the wave's largest y.
+// 2^z for z <= 0 (0 below 2^-1074): 2^n of the nearest whole number times the series of 2^r = e^(r ln 2), |r| <= 1/2, whose rest after
+// the 11th power is below 7e-15 of the value.
+__device__ __forceinline__ double power_of_two(double z) {
+    z = fmax(z, -1080.);
+    const double n = rint(z), r = z - n;
+    double p = 4.4455382718708116e-10;
+    p = fma(p, r, 7.054911620801123e-09);
+    p = fma(p, r, 1.01780860092397e-07);
+    p = fma(p, r, 1.321548679014431e-06);
+    p = fma(p, r, 1.5252733804059841e-05);
+    p = fma(p, r, 0.0001540353039338161);
+    p = fma(p, r, 0.0013333558146428443);
+    p = fma(p, r, 0.009618129107628477);
+    p = fma(p, r, 0.05550410866482158);
+    p = fma(p, r, 0.24022650695910072);
+    p = fma(p, r, 0.6931471805599453);
+    p = fma(p, r, 1.);
+    return ldexp(p, (int)n);
+}
+
+// e[k][j] = 2^(z - m) of the thread's elements (0 where not allowed), m the wave's largest z, which is returned: NaN if a value that is
+// allowed is NaN.
 template <typename T, int K, int ROWS, bool HIST, int VEC>
 __device__ __forceinline__ double exp_values(const Unit<T, K, ROWS, HIST> &u, double (&e)[K][VEC]) {
-    const Rule<double> rule(u.w);
+    const Rule<double> rule(u.w, LOG2E64);
     double m = NEG64;
+    bool bad = false;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const int left = u.left(k), i = u.p.base() + u.p.at(k);
         const uint32_t bits = u.bits(k);
-        float b[VEC];
-        load_bias<VEC>(u.w.bias ? u.w.bias + i : nullptr, left, b);
+        u.values(k, rule, e[k]);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-            e[k][j] = j < left && ((bits >> j) & 1u) ? rule.value((double)(float)u.x[k].v[j], u.count(k, j), (double)b[j]) : NEG64;
+            e[k][j] = select(bit_word(bits, j), e[k][j], NEG64);
+            bad |= e[k][j] != e[k][j];
             m = fmax(m, e[k][j]);
         }
     }
     m = wave_max(m);
+    const double from = m == NEG64 ? 0. : m;
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) e[k][j] = e[k][j] == NEG64 ? 0. : exp(e[k][j] - m);
-    return m;
+        for (int j = 0; j < VEC; ++j) e[k][j] = power_of_two(e[k][j] - from);
+    return __ballot(bad) ? __builtin_nan("") : m;
 }
 
 // The first element, in index order, at which the running sum (starting from `before`) exceeds thr; the last positive one if it never
-// does.  Returns its index inside the wave's piece (or -1: nothing positive) and its e.  The whole wave calls it.
-template <int K, int VEC> __device__ __forceinline__ int pick_in_wave(const double (&e)[K][VEC], int lane, double before, double thr, double *value) {
-    int found = -1, last = -1;
-    double cum = before, v_found = 0., v_last = 0.;
+// does.  Returns whether it did, the element's index inside the wave's piece (-1: nothing positive) and its e.  The whole wave calls it.
+struct Pick {
+    double value;
+    int index;
+    bool over;
+};
+template <int K, int VEC> __device__ __forceinline__ Pick pick_in_wave(const double (&e)[K][VEC], double before, double thr) {
+    Pick found = {0., -1, false};
+    double cum = before;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         double s = 0.;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) s += e[k][j];
-        const double inc = wave_scan(s, lane);
-        // inside the lane: the first positive element past thr, else the last positive one
-        int mine = -1;
-        double run = cum + (inc - s), mine_v = 0.;
-        bool over = false;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j)
-            if (e[k][j] > 0. && !over) run += e[k][j], mine = j, mine_v = e[k][j], over = run > thr;
+        const double inc = wave_scan(s);
         const unsigned long long some = __ballot(s > 0.), hit = __ballot(s > 0. && cum + inc > thr);
-        if (found < 0 && hit) {
-            const int l = __ffsll((long long)hit) - 1;
-            found = (k * 64 + l) * VEC + __shfl(mine, l), v_found = __shfl(mine_v, l);
+        if (!found.over && some) {
+            // inside each lane: the first positive element past thr, else the last positive one
+            int mine = -1;
+            double run = cum + (inc - s), v = 0.;
+            bool over = false;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                if (e[k][j] > 0. && !over) run += e[k][j], mine = j, v = e[k][j], over = run > thr;
+            const int l = hit ? __ffsll((long long)hit) - 1 : 63 - __clzll((long long)some);
+            found.index = (k * 64 + l) * VEC + __builtin_amdgcn_readlane(mine, l), found.value = from_lane(v, l), found.over = hit != 0;
         }
-        if (some) {
-            const int l = 63 - __clzll((long long)some);
-            last = (k * 64 + l) * VEC + __shfl(mine, l), v_last = __shfl(mine_v, l);
-        }
-        cum += __shfl(inc, 63);
+        cum += from_lane(inc, 63);
     }
-    *value = found >= 0 ? v_found : v_last;
-    return found >= 0 ? found : last;
+    return found;
 }
+
+__device__ __forceinline__ float draw_log_prob(double value, double total) { return (float)log(value / total); }
 
 // a whole row in a wave
 template <typename T, int K, int ROWS, bool HIST>
@@ -461,18 +569,15 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(Args a, const float *__res
     const double m = exp_values(u, e);
     double s = 0.;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        double t = 0.;
+    for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int j = 0; j < U::VEC; ++j) t += e[k][j];
-        s += wave_sum(t);
-    }
-    double v;
-    const int pick = pick_in_wave(e, u.p.lane, 0., (double)uniforms[u.p.r * ld_u] * s, &v);
+        for (int j = 0; j < U::VEC; ++j) s += e[k][j];
+    s = wave_sum(s);
+    const Pick pick = pick_in_wave(e, 0., (double)uniforms[u.p.r * ld_u] * s);
     if (u.p.lane == 0) {
-        const bool ok = s > 0. && m < __builtin_inf() && pick >= 0;
-        out[u.p.r] = ok ? pick : empty;
-        lp[u.p.r] = ok ? (float)log(v / s) : (m == NEG64 && s == 0. ? NEG : __builtin_nanf(""));
+        const bool ok = s > 0. && m < __builtin_inf() && pick.index >= 0;
+        out[u.p.r] = ok ? pick.index : empty;
+        lp[u.p.r] = ok ? draw_log_prob(pick.value, s) : (m == NEG64 ? NEG : __builtin_nanf(""));
     }
 }
 
@@ -492,73 +597,87 @@ __global__ __launch_bounds__(NT) void draw_piece_kernel(Args a, Piece *__restric
     if (u.p.lane == 0) part[(long long)u.p.r * a.units * WAVES + u.p.unit * WAVES + u.p.wave] = Piece{s, m};
 }
 
-// One workgroup per row: the pieces joined in index order, the piece that holds u * total found, and its elements walked again (the
-// workgroup counts the piece's ids, its first wave walks).
+// One workgroup per row: the pieces joined in index order, the piece that holds u * total found, and its elements computed and walked
+// again, a slab of it for each wave.
 template <typename T, int K, bool HIST>
 __global__ __launch_bounds__(NT) void draw_join_kernel(Args a, const Piece *__restrict__ part, const float *__restrict__ uniforms,
                                                        long long ld_u, int64_t empty, int64_t *__restrict__ out,
                                                        float *__restrict__ lp) {
-    constexpr int VEC = Elem<T>::VEC, SPAN = 64 * VEC * K;   // a piece: what one wave of draw_piece_kernel had
+    constexpr int VEC = Elem<T>::VEC, SPAN = 64 * VEC * K;             // a piece: what one wave of draw_piece_kernel had
+    constexpr int SLABS = K < WAVES ? 1 : K / WAVES, USED = K / SLABS;   // packs for each of the waves that take part
     __shared__ __align__(16) int cnt[HIST ? SPAN : 4];
-    const int r = blockIdx.x, lane = threadIdx.x & 63, pieces = a.units * WAVES;
+    __shared__ double sums[WAVES];
+    __shared__ Pick picks[WAVES];
+    const int r = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), pieces = a.units * WAVES;
     const Piece *p = part + (long long)r * pieces;
     double m = NEG64;
-    for (int i = lane; i < pieces; i += 64) m = fmax(m, p[i].m);
+    bool bad = false;
+    for (int i = lane; i < pieces; i += 64) m = fmax(m, p[i].m), bad |= p[i].m != p[i].m;
     m = wave_max(m);
+    const bool nan = __ballot(bad) != 0;
+    if (nan || !(m > NEG64 && m < __builtin_inf())) {   // (the same in every wave)
+        if (threadIdx.x == 0) out[r] = empty, lp[r] = !nan && m == NEG64 ? NEG : __builtin_nanf("");
+        return;
+    }
     double total = 0.;
     for (int base = 0; base < pieces; base += 64) {
         const int i = base + lane;
-        const double w = i < pieces ? (p[i].m == NEG64 ? p[i].s : p[i].s * exp(p[i].m - m)) : 0.;
-        total += wave_sum(w);
+        total += wave_sum(i < pieces ? p[i].s * power_of_two(p[i].m - m) : 0.);
     }
-    // every wave of the workgroup has the same total and comes to the same piece
+    // every wave has the same total and comes to the same piece
     const double thr = (double)uniforms[r * ld_u] * total;
-    int found = -1, last = -1;
-    double cum = 0., before = 0., before_last = 0.;
-    for (int base = 0; base < pieces; base += 64) {
+    int found = 0;
+    bool over = false;
+    double cum = 0., before = 0.;
+    for (int base = 0; base < pieces && !over; base += 64) {
         const int i = base + lane;
-        const double w = i < pieces ? (p[i].m == NEG64 ? p[i].s : p[i].s * exp(p[i].m - m)) : 0.;
-        const double inc = wave_scan(w, lane);
+        const double w = i < pieces ? p[i].s * power_of_two(p[i].m - m) : 0.;
+        const double inc = wave_scan(w), ahead = cum + (inc - w);
         const unsigned long long some = __ballot(w > 0.), hit = __ballot(w > 0. && cum + inc > thr);
-        const double ahead = cum + (inc - w);
-        if (found < 0 && hit) {
-            const int l = __ffsll((long long)hit) - 1;
-            found = base + l, before = __shfl(ahead, l);
-        }
         if (some) {
-            const int l = 63 - __clzll((long long)some);
-            last = base + l, before_last = __shfl(ahead, l);
+            const int l = hit ? __ffsll((long long)hit) - 1 : 63 - __clzll((long long)some);
+            found = base + l, before = from_lane(ahead, l), over = hit != 0;
         }
-        cum += __shfl(inc, 63);
-    }
-    if (found < 0) found = last, before = before_last;
-    if (!(total > 0.) || !(m < __builtin_inf()) || found < 0) {
-        if (threadIdx.x == 0) out[r] = empty, lp[r] = m == NEG64 && total == 0. ? NEG : __builtin_nanf("");
-        return;   // (the whole workgroup: every thread has the same total, m and found)
+        cum += from_lane(inc, 63);
     }
     const Row<T> w = row_of<T>(a, r);
-    const int base = found * SPAN, n = a.V - base < SPAN ? a.V - base : SPAN;
+    const int base = found * SPAN, n = a.V - base < SPAN ? a.V - base : SPAN;   // (a piece with a positive sum begins inside the row)
     if (HIST) count_unit(cnt, SPAN, w.hist, w.len, base, n, threadIdx.x, NT);
-    if (threadIdx.x >= 64) return;
-    const Rule<double> rule(w);
-    double e[K][VEC];
+    double e[SLABS][VEC];
+    double s = 0.;
+    if (wave < USED) {
+        const Rule<double> rule(w, LOG2E64);
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        const int at = (k * 64 + lane) * VEC, left = n - at, i = base + at;
-        const Pack<T> x = load_pack(w.x + i, left);
-        const uint32_t bits = left > 0 ? mask_bits<VEC>(w.mask, i) : 0u;
-        float b[VEC];
-        load_bias<VEC>(w.bias ? w.bias + i : nullptr, left, b);
+        for (int k = 0; k < SLABS; ++k) {
+            const int at = ((wave * SLABS + k) * 64 + lane) * VEC, left = n - at, i = base + at;
+            const Pack<T> x = load_pack(w.x + i, left);
+            const uint32_t bits = left > 0 ? (w.mask ? w.mask[i >> 5] >> (i & 31) : 0xffffffffu) : 0u;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j)
-            e[k][j] = j < left && ((bits >> j) & 1u)
-                          ? exp(rule.value((double)(float)x.v[j], HIST ? cnt[at + j] : 0, (double)b[j]) - m) : 0.;
+            for (int j = 0; j < VEC; ++j) {
+                e[k][j] = 0.;
+                if (j < left && ((bits >> j) & 1u)) {
+                    const double y = rule.penalised((double)(float)x.v[j], HIST ? cnt[at + j] : 0) + (w.bias ? (double)w.bias[i + j] : 0.);
+                    e[k][j] = power_of_two(scaled(y, rule.scale) - m);
+                }
+                s += e[k][j];
+            }
+        }
+        s = wave_sum(s);
+        if (lane == 0) sums[wave] = s;
     }
-    double v;
-    const int pick = pick_in_wave(e, lane, before, thr, &v);
-    if (lane == 0) {
-        out[r] = pick >= 0 ? base + pick : empty;
-        lp[r] = pick >= 0 ? (float)log(v / total) : __builtin_nanf("");
+    __syncthreads();
+    if (wave < USED) {
+        for (int v = 0; v < wave; ++v) before += sums[v];
+        const Pick pick = pick_in_wave(e, before, thr);
+        if (lane == 0) picks[wave] = pick;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        Pick best = {0., -1, false};
+        for (int v = 0; v < USED && !best.over; ++v)
+            if (picks[v].index >= 0) best = picks[v], best.index += v * SLABS * 64 * VEC;
+        out[r] = best.index >= 0 ? base + best.index : empty;
+        lp[r] = best.index >= 0 ? draw_log_prob(best.value, total) : __builtin_nanf("");
     }
 }
 
