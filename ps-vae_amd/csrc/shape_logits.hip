@@ -13,7 +13,9 @@
 // large as the logits - and the logits are requested before the walk, so that it runs while they travel.
 #include "common.h"
 
+#include <limits.h>
 #include <math.h>
+#include <type_traits>
 
 namespace {
 
@@ -86,19 +88,6 @@ template <typename T> __device__ __forceinline__ Row<T> row_of(const Args &a, in
         if (s >= 0 && s < a.S) w.mask = (const uint32_t *)a.allowed + s * a.ld_allowed;
     }
     return w;
-}
-
-// Counts of the ids [base, base + n) in the row's history, into cnt[0 .. n).  Every thread of the workgroup calls it (barriers);
-// the calling group's threads number `tid` of `threads`.
-__device__ __forceinline__ void count_unit(int *cnt, int span, const int64_t *hist, int len, int base, int n, int tid, int threads) {
-    for (int i = tid * 4; i < span; i += threads * 4) *reinterpret_cast<int4 *>(cnt + i) = make_int4(0, 0, 0, 0);
-    __syncthreads();
-#pragma unroll 4
-    for (int j = tid; j < len; j += threads) {
-        const unsigned long long at = (unsigned long long)(hist[j] - base);   // ids outside the vocabulary fall outside every unit
-        if (at < (unsigned long long)n) atomicAdd(&cnt[at], 1);
-    }
-    __syncthreads();
 }
 
 // VEC values from p[0 .. left): the whole 16 bytes where they are inside, one by one at a row's end.
@@ -175,14 +164,26 @@ template <typename C> __device__ __forceinline__ C wave_max(C v) {
     return from_lane(v, 63);
 }
 
+// 1 / x by Newton's iteration from the unit's estimate (1 ulp; 2^-22 for doubles): a row's few reciprocals cost 3 and 5 instructions
+// instead of a division's 10 and 14.
+__device__ __forceinline__ float reciprocal(float x) {
+    const float r = __builtin_amdgcn_rcpf(x);
+    return fmaf(fmaf(-x, r, 1.f), r, r);
+}
+__device__ __forceinline__ double reciprocal(double x) {
+    double r = __builtin_amdgcn_rcp(x);
+    r = fma(fma(-x, r, 1.), r, r);
+    return fma(fma(-x, r, 1.), r, r);
+}
+
 // The penalties and the last factor of a row in type C (float; double for draws).  `unit` scales the result: 1, or log2 e where it goes
 // into a power of two.
 template <typename C> struct Rule {
     C rep, inv_rep, pres, freq, scale;
     template <typename T> __device__ Rule(const Row<T> &w, C unit)
-        : rep((C)w.rep), inv_rep((C)1 / (C)w.rep), pres((C)w.pres), freq((C)w.freq), scale(unit / (C)w.temp) {}
+        : rep((C)w.rep), inv_rep(reciprocal((C)w.rep)), pres((C)w.pres), freq((C)w.freq), scale(unit * reciprocal((C)w.temp)) {}
     __device__ __forceinline__ C factor(C x) const { return x > (C)0 ? inv_rep : rep; }   // what a seen token's logit is multiplied by
-    __device__ __forceinline__ C penalised(C x, int c) const { return c > 0 ? x * factor(x) - (freq * (C)c + pres) : x; }
+    __device__ __forceinline__ C penalised(C x, int c) const { return x * factor(x) - (freq * (C)c + pres); }
 };
 
 // y in units of 1 / scale, rounded by itself.  Equal values have to stay equal: fused with the subtraction of the row's maximum that follows, the
@@ -226,87 +227,168 @@ template <typename T, int K, int ROWS> struct Place {
     __device__ __forceinline__ int at(int k) const { return ((wave * K + k) * 64 + lane) * VEC; }   // inside the unit
 };
 
-// Loads a thread's logits, counts the unit, and hands out what belongs to pack k of it.
-template <typename T, int K, int ROWS, bool HIST> struct Unit {
+// What the past does to a unit: the count of every id in `cell`, and one bit for every id that occurs in `seen`.
+template <int SPAN> struct Past {
+    int cell[SPAN];
+    uint32_t seen[SPAN / 32];
+};
+struct NoPast {};
+
+// Counts the ids [base, base + n) of the row's history.  Every thread of the workgroup calls it (barriers); the calling group's threads
+// number `tid` of `threads`.
+template <int SPAN>
+__device__ __forceinline__ void count_unit(Past<SPAN> &past, const int64_t *hist, int len, int base, int n, int tid, int threads) {
+    for (int i = tid * 4; i < SPAN; i += threads * 4) *reinterpret_cast<int4 *>(past.cell + i) = make_int4(0, 0, 0, 0);
+    for (int i = tid; i < SPAN / 32; i += threads) past.seen[i] = 0u;
+    __syncthreads();
+#pragma unroll 4
+    for (int j = tid; j < len; j += threads) {
+        const unsigned long long at = (unsigned long long)(hist[j] - base);   // ids outside the vocabulary fall outside every unit
+        if (at < (unsigned long long)n) {
+            atomicAdd(&past.cell[at], 1);
+            atomicOr(&past.seen[at >> 5], 1u << (at & 31));
+        }
+    }
+    __syncthreads();
+}
+
+// A thread's part of a unit: K packs of logits with their bias and mask, requested before the history is walked, and what the walk found.
+//   PAST 0: no history.  1: counts (and bits).  2: `cell` holds the finished value y of every seen id in place of its count, computed
+//   once by one thread; a pack of 64 * VEC ids that has a seen one then costs two instructions an element more, not eight.
+template <typename T, int K, int ROWS, int PAST> struct Unit {
     using P = Place<T, K, ROWS>;
+    using Lds = std::conditional_t<PAST != 0, Past<P::SPAN>, NoPast>;
     static constexpr int VEC = P::VEC;
     P p;
     Row<T> w;
     Pack<T> x[K];
-    int *cnt;
+    float b[K][VEC];
+    uint32_t allow[K];               // bit j: element j of the pack is in the row and allowed
+    Lds *past;
     int n;                           // elements of the unit that the row has
-    __device__ Unit(const Args &a, int block, int *lds, bool want_logits) : p(a, block), w(row_of<T>(a, p.r)) {
-        const int base = p.base();
-        n = p.live ? (a.V - base < P::SPAN ? a.V - base : P::SPAN) : 0;
-        if (want_logits) {
-            if (n == P::SPAN) {      // (no lane's load hangs on a test of its own)
-#pragma unroll
-                for (int k = 0; k < K; ++k) x[k] = *reinterpret_cast<const Pack<T> *>(w.x + base + p.at(k));
-            } else {
-#pragma unroll
-                for (int k = 0; k < K; ++k) x[k] = load_pack(w.x + base + p.at(k), n - p.at(k));
-            }
-        }
-        cnt = HIST ? lds + (ROWS == 1 ? 0 : (int)threadIdx.x / P::THREADS * P::SPAN) : nullptr;
-        if (HIST) count_unit(cnt, P::SPAN, w.hist, p.live ? w.len : 0, base, n, p.tid, P::THREADS);
-    }
+
     __device__ __forceinline__ int left(int k) const { return n - p.at(k); }
     __device__ __forceinline__ int element(int k) const { return p.base() + p.at(k); }
-    // bit j: element j of the pack is in the row and allowed
-    __device__ __forceinline__ uint32_t bits(int k) const {
-        const int l = left(k);
-        if (w.none || l <= 0) return 0u;
-        const int i = element(k);
-        const uint32_t b = w.mask ? w.mask[i >> 5] >> (i & 31) : 0xffffffffu;   // (i is a multiple of VEC: one word)
-        return l >= VEC ? b : b & ((1u << l) - 1u);
-    }
-    // the counts of the pack; whether any lane of the wave has one above 0
-    __device__ __forceinline__ bool counts(int k, int (&c)[VEC]) const {
-        int any = 0;
+    __device__ Unit(const Args &a, int block, Lds *lds, bool want_logits) : p(a, block), w(row_of<T>(a, p.r)) {
+        const int base = p.base();
+        n = p.live ? (a.V - base < P::SPAN ? a.V - base : P::SPAN) : 0;
+        past = lds + (ROWS == 1 ? 0 : (int)threadIdx.x / P::THREADS);
 #pragma unroll
-        for (int q = 0; q < VEC / 4; ++q) {
-            const int4 v = *reinterpret_cast<const int4 *>(cnt + p.at(k) + 4 * q);
-            c[4 * q] = v.x, c[4 * q + 1] = v.y, c[4 * q + 2] = v.z, c[4 * q + 3] = v.w;
-            any |= (v.x | v.y) | (v.z | v.w);
+        for (int k = 0; k < K; ++k) {
+            allow[k] = 0xffffffffu;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) b[k][j] = 0.f;
         }
-        return __ballot(any != 0) != 0;
-    }
-    // y of the pack, before the mask
-    template <typename C> __device__ __forceinline__ void values(int k, const Rule<C> &rule, C (&y)[VEC]) const {
+        if (n == P::SPAN) {          // (no lane's load hangs on a test of its own)
+            if (want_logits) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) y[j] = (C)(float)x[k].v[j];
-        if (HIST) {
-            int c[VEC];
-            if (counts(k, c)) {
+                for (int k = 0; k < K; ++k) x[k] = *reinterpret_cast<const Pack<T> *>(w.x + element(k));
+                if (w.bias) {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) y[j] = rule.penalised(y[j], c[j]);
+                    for (int k = 0; k < K; ++k) load_bias<VEC>(w.bias + element(k), VEC, b[k]);
+                }
+            }
+            if (w.mask) {
+#pragma unroll
+                for (int k = 0; k < K; ++k) allow[k] = w.mask[element(k) >> 5] >> (element(k) & 31);   // (whole packs: one word)
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const int l = left(k);
+                if (want_logits) {
+                    x[k] = load_pack(w.x + element(k), l);
+                    if (w.bias) load_bias<VEC>(w.bias + element(k), l, b[k]);
+                }
+                if (w.mask && l > 0) allow[k] = w.mask[element(k) >> 5] >> (element(k) & 31);
+                allow[k] &= l >= VEC ? 0xffffffffu : l > 0 ? (1u << l) - 1u : 0u;
             }
         }
-        if (w.bias) {
-            float b[VEC];
-            load_bias<VEC>(w.bias + element(k), left(k), b);
+        if (w.none) {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) y[j] += (C)b[j];
+            for (int k = 0; k < K; ++k) allow[k] = 0u;
+        }
+        if constexpr (PAST != 0) count_unit(*past, w.hist, p.live ? w.len : 0, base, n, p.tid, P::THREADS);
+    }
+    // PAST 2: one thread for each seen id - the one that takes its bit - leaves y in its cell; the bits are set again as they are taken.
+    __device__ __forceinline__ void finish_seen(const Rule<float> &rule) {
+        for (int i = p.tid; i < P::SPAN / 32; i += P::THREADS) past->seen[i] = 0u;
+        __syncthreads();
+        const int base = p.base(), len = p.live ? w.len : 0;
+#pragma unroll 4
+        for (int j = p.tid; j < len; j += P::THREADS) {
+            const unsigned long long at = (unsigned long long)(w.hist[j] - base);
+            if (at < (unsigned long long)n) {
+                const uint32_t bit = 1u << (at & 31);
+                if (!(atomicOr(&past->seen[at >> 5], bit) & bit)) {
+                    const int i = base + (int)at;
+                    const float v = rule.penalised((float)w.x[i], past->cell[at]) + (w.bias ? w.bias[i] : 0.f);
+                    past->cell[at] = __float_as_int(scaled(v, rule.scale));
+                }
+            }
+        }
+        __syncthreads();
+    }
+    // bit j: element j of pack k has been seen; 0 in every lane unless one of the wave has a bit
+    __device__ __forceinline__ uint32_t seen(int k) const {
+        if constexpr (PAST == 0) return 0u;
+        else return (reinterpret_cast<const uint8_t *>(past->seen)[p.at(k) >> 3] >> (p.at(k) & 7)) & ((1u << VEC) - 1u);
+    }
+    __device__ __forceinline__ void cells(int k, int (&c)[VEC]) const {
+        if constexpr (PAST != 0) {
+#pragma unroll
+            for (int q = 0; q < VEC / 4; ++q) {
+                const int4 v = *reinterpret_cast<const int4 *>(past->cell + p.at(k) + 4 * q);
+                c[4 * q] = v.x, c[4 * q + 1] = v.y, c[4 * q + 2] = v.z, c[4 * q + 3] = v.w;
+            }
+        }
+    }
+    // y of pack k, before the mask
+    __device__ __forceinline__ void values(int k, const Rule<float> &rule, float (&y)[VEC]) const {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) y[j] = scaled((float)x[k].v[j] + b[k][j], rule.scale);
+        if (PAST == 2) {
+            const uint32_t s = seen(k);
+            if (__ballot(s != 0)) {
+                int c[VEC];
+                cells(k, c);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) y[j] = select(bit_word(s, j), __int_as_float(c[j]), y[j]);
+            }
+        }
+    }
+    __device__ __forceinline__ void values(int k, const Rule<double> &rule, double (&y)[VEC]) const {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) y[j] = (double)(float)x[k].v[j];
+        if (PAST == 1) {
+            const uint32_t s = seen(k);
+            if (__ballot(s != 0)) {
+                int c[VEC];
+                cells(k, c);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    if (c[j] > 0) y[j] = rule.penalised(y[j], c[j]);
+            }
         }
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) y[j] = scaled(y[j], rule.scale);
+        for (int j = 0; j < VEC; ++j) y[j] = scaled(y[j] + (double)b[k][j], rule.scale);
     }
 };
 
 template <typename T, int K, int ROWS, bool HIST>
 __global__ __launch_bounds__(NT) void shape_fwd_kernel(Args a, T *__restrict__ out, long long ld_out) {
-    using U = Unit<T, K, ROWS, HIST>;
-    __shared__ __align__(16) int lds[HIST ? U::P::SPAN * ROWS : 4];
+    using U = Unit<T, K, ROWS, HIST ? 2 : 0>;
+    __shared__ __align__(16) typename U::Lds lds[ROWS];
     U u(a, blockIdx.x, lds, true);
     const Rule<float> rule(u.w, 1.f);
+    if constexpr (HIST) u.finish_seen(rule);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const uint32_t bits = u.bits(k);
         float v[U::VEC];
         u.values(k, rule, v);
         Pack<T> y;
 #pragma unroll
-        for (int j = 0; j < U::VEC; ++j) y.v[j] = (T)select(bit_word(bits, j), v[j], NEG);
+        for (int j = 0; j < U::VEC; ++j) y.v[j] = (T)select(bit_word(u.allow[k], j), v[j], NEG);
         store_pack(out + u.p.r * ld_out + u.element(k), y, u.left(k));
     }
 }
@@ -315,31 +397,31 @@ __global__ __launch_bounds__(NT) void shape_fwd_kernel(Args a, T *__restrict__ o
 template <typename T, int K, int ROWS, bool HIST>
 __global__ __launch_bounds__(NT) void shape_bwd_kernel(Args a, const T *__restrict__ g, long long ld_gb, long long ld_gt,
                                                        T *__restrict__ dx, long long ld_dx) {
-    using U = Unit<T, K, ROWS, HIST>;
-    __shared__ __align__(16) int lds[HIST ? U::P::SPAN * ROWS : 4];
+    using U = Unit<T, K, ROWS, HIST ? 1 : 0>;
+    __shared__ __align__(16) typename U::Lds lds[ROWS];
     U u(a, blockIdx.x, lds, false);
     const Rule<float> rule(u.w, 1.f);
     const int b = a.T == 1 ? u.p.r : (int)((unsigned)u.p.r / (unsigned)a.T), t = u.p.r - b * a.T;
     const T *gr = g + b * ld_gb + t * ld_gt;
 #pragma unroll
+    for (int k = 0; k < K; ++k) u.x[k] = load_pack(gr + u.element(k), u.left(k));
+#pragma unroll
     for (int k = 0; k < K; ++k) {
-        const uint32_t bits = u.bits(k);
         const int i = u.element(k);
-        const Pack<T> gv = load_pack(gr + i, u.left(k));
         float v[U::VEC];
 #pragma unroll
-        for (int j = 0; j < U::VEC; ++j) v[j] = (float)gv.v[j] * rule.scale;
+        for (int j = 0; j < U::VEC; ++j) v[j] = (float)u.x[k].v[j] * rule.scale;
         if (HIST) {
-            int c[U::VEC];
-            if (u.counts(k, c)) {
+            const uint32_t s = u.seen(k);
+            if (__ballot(s != 0)) {
 #pragma unroll
                 for (int j = 0; j < U::VEC; ++j)
-                    if (c[j] > 0) v[j] *= rule.factor((float)u.w.x[i + j]);
+                    if ((s >> j) & 1u) v[j] *= rule.factor((float)u.w.x[i + j]);
             }
         }
         Pack<T> d;
 #pragma unroll
-        for (int j = 0; j < U::VEC; ++j) d.v[j] = (T)select(bit_word(bits, j), v[j], 0.f);
+        for (int j = 0; j < U::VEC; ++j) d.v[j] = (T)select(bit_word(u.allow[k], j), v[j], 0.f);
         store_pack(dx + u.p.r * ld_dx + i, d, u.left(k));
     }
 }
@@ -347,6 +429,9 @@ __global__ __launch_bounds__(NT) void shape_bwd_kernel(Args a, const T *__restri
 __device__ __forceinline__ float log_prob_of(float y_tok, float m, float s) {
     return m == NEG && s == 0.f ? NEG : y_tok - m - logf(s);   // (nothing allowed: log 0)
 }
+
+// a row's token as an element of it, or one that no pack holds
+__device__ __forceinline__ int token_of(long long tok, int V) { return tok >= 0 && tok < V ? (int)tok : INT_MIN / 2; }
 
 // exp(y - m) as a power of two.  (The difference first: a row of the type's lowest values - masked by hand - has an m whose multiple of
 // log2 e overflows.)  A piece that allows nothing has m = -inf: 0 in its place.
@@ -361,30 +446,30 @@ template <typename T, int K, int ROWS, bool HIST>
 __global__ __launch_bounds__(NT) void log_prob_fwd_kernel(Args a, const int64_t *__restrict__ tokens, float *__restrict__ lp,
                                                           float2 *__restrict__ stats, float2 *__restrict__ part,
                                                           float *__restrict__ target) {
-    using U = Unit<T, K, ROWS, HIST>;
-    __shared__ __align__(16) int lds[HIST ? U::P::SPAN * ROWS : 4];
+    using U = Unit<T, K, ROWS, HIST ? 2 : 0>;
+    __shared__ __align__(16) typename U::Lds lds[ROWS];
     U u(a, blockIdx.x, lds, true);
-    if (!u.p.live) return;
     const Rule<float> rule(u.w, 1.f);
-    const long long tok = tokens[u.p.r];
+    if constexpr (HIST) u.finish_seen(rule);
+    if (!u.p.live) return;
+    const int tok = token_of(tokens[u.p.r], a.V);
     float y[K][U::VEC];
     float m = NEG, yt = 0.f;
     bool mine = false;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const uint32_t bits = u.bits(k);
         u.values(k, rule, y[k]);
 #pragma unroll
         for (int j = 0; j < U::VEC; ++j) {
-            y[k][j] = select(bit_word(bits, j), y[k][j], NEG);
+            y[k][j] = select(bit_word(u.allow[k], j), y[k][j], NEG);
             m = fmaxf(m, y[k][j]);
         }
-        const long long at = tok - u.element(k);
-        if (at >= 0 && at < U::VEC && at < u.left(k)) {
+        const unsigned at = (unsigned)(tok - u.element(k));
+        if (at < (unsigned)U::VEC) {
             mine = true;
 #pragma unroll
             for (int j = 0; j < U::VEC; ++j)
-                if (j == at) yt = y[k][j];
+                if (j == (int)at) yt = y[k][j];
         }
     }
     m = wave_max(m);
@@ -430,36 +515,36 @@ __global__ __launch_bounds__(NT) void log_prob_join_kernel(int R, int V, int pie
 template <typename T, int K, int ROWS, bool HIST>
 __global__ __launch_bounds__(NT) void log_prob_bwd_kernel(Args a, const int64_t *__restrict__ tokens, const float2 *__restrict__ stats,
                                                           const float *__restrict__ g, T *__restrict__ dx, long long ld_dx) {
-    using U = Unit<T, K, ROWS, HIST>;
-    __shared__ __align__(16) int lds[HIST ? U::P::SPAN * ROWS : 4];
+    using U = Unit<T, K, ROWS, HIST ? 2 : 0>;
+    __shared__ __align__(16) typename U::Lds lds[ROWS];
     U u(a, blockIdx.x, lds, true);
     const Rule<float> rule(u.w, 1.f);
-    const long long tok = tokens[u.p.r];
+    if constexpr (HIST) u.finish_seen(rule);
+    const int tok = token_of(tokens[u.p.r], a.V);
     const float2 st = stats[u.p.r];
-    const bool zero = tok < 0 || tok >= a.V || (st.x == NEG && st.y == 0.f);   // a row without a token, or with none allowed
+    const bool zero = tok < 0 || (st.x == NEG && st.y == 0.f);   // a row without a token, or with none allowed
     const float at_token = g[u.p.r] * rule.scale, others = -at_token / st.y, from = reference_of(st.x);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const uint32_t bits = zero ? 0u : u.bits(k);
         const int i = u.element(k);
         float v[U::VEC];
         u.values(k, rule, v);
 #pragma unroll
         for (int j = 0; j < U::VEC; ++j) v[j] = others * exp_from(v[j], from);
-        const long long at = tok - i;
-        if (at >= 0 && at < U::VEC) {
+        const unsigned at = (unsigned)(tok - i);
+        if (at < (unsigned)U::VEC) {
 #pragma unroll
             for (int j = 0; j < U::VEC; ++j)
-                if (j == at) v[j] += at_token;
+                if (j == (int)at) v[j] += at_token;
         }
         if (HIST) {
-            int c[U::VEC];
-            if (u.counts(k, c)) {
+            const uint32_t s = u.seen(k);
+            if (__ballot(s != 0)) {
 #pragma unroll
-                for (int j = 0; j < U::VEC; ++j)
-                    if (c[j] > 0) v[j] *= rule.factor((float)u.x[k].v[j]);
+                for (int j = 0; j < U::VEC; ++j) v[j] = select(bit_word(s, j), v[j] * rule.factor((float)u.x[k].v[j]), v[j]);
             }
         }
+        const uint32_t bits = zero ? 0u : u.allow[k];
         Pack<T> d;
 #pragma unroll
         for (int j = 0; j < U::VEC; ++j) d.v[j] = (T)select(bit_word(bits, j), v[j], 0.f);
@@ -497,18 +582,17 @@ __device__ __forceinline__ double power_of_two(double z) {
 
 // e[k][j] = 2^(z - m) of the thread's elements (0 where not allowed), m the wave's largest z, which is returned: NaN if a value that is
 // allowed is NaN.
-template <typename T, int K, int ROWS, bool HIST, int VEC>
-__device__ __forceinline__ double exp_values(const Unit<T, K, ROWS, HIST> &u, double (&e)[K][VEC]) {
+template <typename T, int K, int ROWS, int PAST, int VEC>
+__device__ __forceinline__ double exp_values(const Unit<T, K, ROWS, PAST> &u, double (&e)[K][VEC]) {
     const Rule<double> rule(u.w, LOG2E64);
     double m = NEG64;
     bool bad = false;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const uint32_t bits = u.bits(k);
         u.values(k, rule, e[k]);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-            e[k][j] = select(bit_word(bits, j), e[k][j], NEG64);
+            e[k][j] = select(bit_word(u.allow[k], j), e[k][j], NEG64);
             bad |= e[k][j] != e[k][j];
             m = fmax(m, e[k][j]);
         }
@@ -561,8 +645,8 @@ __device__ __forceinline__ float draw_log_prob(double value, double total) { ret
 template <typename T, int K, int ROWS, bool HIST>
 __global__ __launch_bounds__(NT) void draw_row_kernel(Args a, const float *__restrict__ uniforms, long long ld_u, int64_t empty,
                                                       int64_t *__restrict__ out, float *__restrict__ lp) {
-    using U = Unit<T, K, ROWS, HIST>;
-    __shared__ __align__(16) int lds[HIST ? U::P::SPAN * ROWS : 4];
+    using U = Unit<T, K, ROWS, HIST ? 1 : 0>;
+    __shared__ __align__(16) typename U::Lds lds[ROWS];
     U u(a, blockIdx.x, lds, true);
     if (!u.p.live) return;
     double e[K][U::VEC];
@@ -583,8 +667,8 @@ __global__ __launch_bounds__(NT) void draw_row_kernel(Args a, const float *__res
 
 template <typename T, int K, bool HIST>
 __global__ __launch_bounds__(NT) void draw_piece_kernel(Args a, Piece *__restrict__ part) {
-    using U = Unit<T, K, 1, HIST>;
-    __shared__ __align__(16) int lds[HIST ? U::P::SPAN : 4];
+    using U = Unit<T, K, 1, HIST ? 1 : 0>;
+    __shared__ __align__(16) typename U::Lds lds[1];
     U u(a, blockIdx.x, lds, true);
     double e[K][U::VEC];
     const double m = exp_values(u, e);
@@ -605,7 +689,7 @@ __global__ __launch_bounds__(NT) void draw_join_kernel(Args a, const Piece *__re
                                                        float *__restrict__ lp) {
     constexpr int VEC = Elem<T>::VEC, SPAN = 64 * VEC * K;             // a piece: what one wave of draw_piece_kernel had
     constexpr int SLABS = K < WAVES ? 1 : K / WAVES, USED = K / SLABS;   // packs for each of the waves that take part
-    __shared__ __align__(16) int cnt[HIST ? SPAN : 4];
+    __shared__ __align__(16) std::conditional_t<HIST, Past<SPAN>, NoPast> past;
     __shared__ double sums[WAVES];
     __shared__ Pick picks[WAVES];
     const int r = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), pieces = a.units * WAVES;
@@ -642,7 +726,7 @@ __global__ __launch_bounds__(NT) void draw_join_kernel(Args a, const Piece *__re
     }
     const Row<T> w = row_of<T>(a, r);
     const int base = found * SPAN, n = a.V - base < SPAN ? a.V - base : SPAN;   // (a piece with a positive sum begins inside the row)
-    if (HIST) count_unit(cnt, SPAN, w.hist, w.len, base, n, threadIdx.x, NT);
+    if constexpr (HIST) count_unit(past, w.hist, w.len, base, n, threadIdx.x, NT);
     double e[SLABS][VEC];
     double s = 0.;
     if (wave < USED) {
@@ -656,8 +740,11 @@ __global__ __launch_bounds__(NT) void draw_join_kernel(Args a, const Piece *__re
             for (int j = 0; j < VEC; ++j) {
                 e[k][j] = 0.;
                 if (j < left && ((bits >> j) & 1u)) {
-                    const double y = rule.penalised((double)(float)x.v[j], HIST ? cnt[at + j] : 0) + (w.bias ? (double)w.bias[i + j] : 0.);
-                    e[k][j] = power_of_two(scaled(y, rule.scale) - m);
+                    double y = (double)(float)x.v[j];
+                    if constexpr (HIST) {
+                        if (past.cell[at + j] > 0) y = rule.penalised(y, past.cell[at + j]);
+                    }
+                    e[k][j] = power_of_two(scaled(y + (w.bias ? (double)w.bias[i + j] : 0.), rule.scale) - m);
                 }
                 s += e[k][j];
             }

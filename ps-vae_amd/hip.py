@@ -711,26 +711,16 @@ def piece_draw(logits, temperature, uniforms_col, pad, end, first_step, piece_at
 
 
 def shape_logits(*shaping):
-    """psvae_shape_logits_fwd; `shaping`: logits, history, history_len, repetition, presence, frequency, temperature
+    """psvae_shape_logits_fwd (differentiable in the logits); `shaping`: logits, history, history_len, repetition, presence, frequency, temperature
     (tensors or None), the four scalars that stand in for them, bias, allowed, state."""
     _count()
     return ops().shape_logits(*shaping)
 
 
-def shape_logits_backward(g, *shaping):
-    _count()
-    return ops().shape_logits_backward(g, *shaping)
-
-
 def shaped_log_prob(tokens, *shaping):
-    """(log-probabilities, stats) of psvae_shaped_log_prob_fwd."""
+    """psvae_shaped_log_prob_fwd (differentiable in the logits)."""
     _count()
     return ops().shaped_log_prob(tokens, *shaping)
-
-
-def shaped_log_prob_backward(g, stats, tokens, *shaping):
-    _count()
-    return ops().shaped_log_prob_backward(g, stats, tokens, *shaping)
 
 
 def shaped_draw(uniforms, empty_token, *shaping):

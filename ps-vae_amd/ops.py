@@ -1024,56 +1024,28 @@ def pack_allowed(allowed):
     return torch.where(words >= 1 << 31, words - (1 << 32), words).to(torch.int32)
 
 
-_NEUTRAL = (1.0, 0.0, 0.0, 1.0)   # repetition, presence, frequency, temperature that change nothing
+def _number_or_rows(v, neutral):
+    """(tensor, number) of a penalty or temperature: one value per sequence, or one number for all."""
+    if v is None:
+        return None, neutral
+    if torch.is_tensor(v):
+        if v.requires_grad:
+            raise ValueError('penalties and temperature are data: none of them gets a gradient')
+        return v, neutral
+    return None, float(v)
 
 
-def _shaping(logits, history, history_len, repetition, presence, frequency, bias, allowed, state, temperature):
-    """The operators' arguments behind the logits, in the order of torch.ops.psvae.shape_logits: a penalty or temperature is
-    either a tensor with one value per sequence or one number for all."""
-    tensors, numbers = [], []
-    for v, neutral in zip((repetition, presence, frequency, temperature), _NEUTRAL):
-        is_tensor = torch.is_tensor(v)
-        tensors.append(v if is_tensor else None)
-        numbers.append(neutral if v is None or is_tensor else float(v))
-    if history is None and (repetition is not None or presence is not None or frequency is not None):
+def _shaping(history, history_len, repetition, presence, frequency, bias, allowed, state, temperature):
+    """The operators' arguments behind the logits, in the order of torch.ops.psvae.shape_logits."""
+    if history is None and not (repetition is None and presence is None and frequency is None):
         raise ValueError('penalties need a history')
-    for t in (bias, *tensors):
-        if t is not None and t.requires_grad and torch.is_grad_enabled():
-            raise ValueError('penalties, bias and temperature are data: none of them gets a gradient')
-    return (history, history_len, *tensors, numbers, bias, allowed, state)
-
-
-class _ShapeLogits(Function):
-    @staticmethod
-    def forward(ctx, logits, *shaping):
-        ctx.save_for_backward(logits, *(t for t in shaping if torch.is_tensor(t)))
-        ctx.shaping = [None if torch.is_tensor(t) else (t,) for t in shaping]   # (None: a saved tensor's place)
-        return hip.shape_logits(logits, *shaping)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
-        saved = iter(ctx.saved_tensors)
-        logits = next(saved)
-        return (hip.shape_logits_backward(g, logits, *(next(saved) if t is None else t[0] for t in ctx.shaping)),
-                *[None] * len(ctx.shaping))
-
-
-class _ShapedLogProb(Function):
-    @staticmethod
-    def forward(ctx, logits, tokens, *shaping):
-        lp, stats = hip.shaped_log_prob(tokens, logits, *shaping)
-        ctx.save_for_backward(logits, tokens, stats, *(t for t in shaping if torch.is_tensor(t)))
-        ctx.shaping = [None if torch.is_tensor(t) else (t,) for t in shaping]
-        return lp
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
-        saved = iter(ctx.saved_tensors)
-        logits, tokens, stats = next(saved), next(saved), next(saved)
-        return (hip.shaped_log_prob_backward(g, stats, tokens, logits, *(next(saved) if t is None else t[0] for t in ctx.shaping)),
-                *[None] * (1 + len(ctx.shaping)))
+    if bias is not None and bias.requires_grad:
+        raise ValueError('the bias is data: it gets no gradient')
+    repetition, r = _number_or_rows(repetition, 1.0)
+    presence, p = _number_or_rows(presence, 0.0)
+    frequency, f = _number_or_rows(frequency, 0.0)
+    temperature, t = _number_or_rows(temperature, 1.0)
+    return history, history_len, repetition, presence, frequency, temperature, (r, p, f, t), bias, allowed, state
 
 
 def shape_logits(logits, *, history=None, history_len=None, repetition=None, presence=None, frequency=None, bias=None,
@@ -1091,9 +1063,7 @@ def shape_logits(logits, *, history=None, history_len=None, repetition=None, pre
     forbidden, past the table: everything is; None: the table has one row for all, or one per sequence.
 
     Differentiable in the logits (once); masked places get no gradient and what they hold is never looked at."""
-    shaping = _shaping(logits, history, history_len, repetition, presence, frequency, bias, allowed, state, temperature)
-    if logits.requires_grad and torch.is_grad_enabled():
-        return _ShapeLogits.apply(logits, *shaping)
+    shaping = _shaping(history, history_len, repetition, presence, frequency, bias, allowed, state, temperature)
     return hip.shape_logits(logits, *shaping)
 
 
@@ -1102,10 +1072,8 @@ def shaped_log_prob(logits, tokens, *, history=None, history_len=None, repetitio
     """log softmax(y)[token] in float32, y as shape_logits shapes it (same arguments; never written out): tokens int64 [B] or
     [B, T], one for each row.  A token outside the vocabulary: 0 and no gradient (padding).  A token that the mask forbids, or a row
     that allows none: -inf (the latter without gradient).  Differentiable in the logits (once)."""
-    shaping = _shaping(logits, history, history_len, repetition, presence, frequency, bias, allowed, state, temperature)
-    if logits.requires_grad and torch.is_grad_enabled():
-        return _ShapedLogProb.apply(logits, tokens, *shaping)
-    return hip.shaped_log_prob(tokens, logits, *shaping)[0]
+    shaping = _shaping(history, history_len, repetition, presence, frequency, bias, allowed, state, temperature)
+    return hip.shaped_log_prob(tokens, logits, *shaping)
 
 
 def shaped_draw(logits, uniforms, *, history=None, history_len=None, repetition=None, presence=None, frequency=None, bias=None,
@@ -1114,5 +1082,5 @@ def shaped_draw(logits, uniforms, *, history=None, history_len=None, repetition=
     probabilities exceeds uniforms[b] (float32 [B] in [0, 1)) times their total.  Returns (tokens int64 [B], log-probabilities
     float32 [B]).  A row that allows no token gives empty_token and -inf, one with NaN or +inf among its allowed values empty_token
     and NaN."""
-    shaping = _shaping(logits, history, history_len, repetition, presence, frequency, bias, allowed, state, temperature)
+    shaping = _shaping(history, history_len, repetition, presence, frequency, bias, allowed, state, temperature)
     return hip.shaped_draw(uniforms, empty_token, logits, *shaping)

@@ -482,6 +482,12 @@ def test_refusals():
         ops.shaped_draw(x, torch.zeros(4, device=d).double())
     with pytest.raises(RuntimeError):
         ops.shaped_draw(x[None], torch.zeros(1, device=d))
+    # no second derivative: an error, not a constant
+    leaf = x.clone().requires_grad_(True)
+    for y in (ops.shape_logits(leaf * leaf), ops.shaped_log_prob(leaf * leaf, torch.zeros(4, dtype=torch.int64, device=d))):
+        first, = torch.autograd.grad(y.sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match='differentiated again'):
+            first.sum().backward()
     # a history written to after the forward pass is noticed by autograd, not silently recounted
     leaf = x.clone().requires_grad_(True)
     y = ops.shape_logits(leaf, history=h, repetition=1.5)
