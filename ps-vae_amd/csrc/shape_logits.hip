@@ -6,16 +6,24 @@
 //     log_prob = y_tok - m - log s,  m = max y, s = sum exp(y - m);  d log_prob / d l_i = ([i = tok] - exp(y_i - m) / s) dy_i/dl_i
 //     draw:  min(#{i : cdf_i <= u cdf_last}, last i of positive probability),  cdf the running sum of exp(y - m) in index order
 //
-// Layout.  A row is cut into units of THREADS * VEC * K elements, a thread's VEC neighbours being one 16-byte load; inside a unit
-// every wave owns a contiguous piece, so a wave's partial results are results of an index range.  The counts c_i of a unit live in
-// LDS only: the unit's threads walk the row's history (8 bytes an entry, from L2 after the row's first unit) and add to 32-bit
-// LDS counters, whose sums do not depend on the order.  No count table of [rows, V] is ever kept or read - it would be as
-// large as the logits - and the logits are requested before the walk, so that it runs while they travel.
+// Bound: one read of the logits (and one write) at large sizes, launches at small ones, with 12 to 25 vector instructions an element in
+// between that have to stay under the time of the loads.
+//
+// Rows of at most 1024 logits: one wave each (Narrow).  Wider rows are cut into runs of up to 32768 elements, a workgroup each, whose
+// waves stream through it in steps of 512 or 1024 elements with the next step's loads in flight (Run).
+//
+// The penalties need c_i.  No table of counts of [rows, V] is kept or read - it would be as large as the logits.  The
+// workgroup walks the row's history itself (8 bytes an entry) and builds in LDS what its elements need: one bit per element says whether the id was
+// seen, and the finished values y of the seen ids - computed once by one thread each - lie in a list in the order of the bits.  The
+// stream over the elements leaves the seen ones out of its sums, or writes them as if nothing had been seen; the list's values are added,
+// or written over these, afterwards.  So an element that was not seen, which nearly all are not, pays nothing for the question (looked up
+// element by element the seen ones cost 8 of 24 instructions).  Counts are sums of integers and every value is computed from them
+// alone: the order of the LDS atomics does not show.
 #include "common.h"
 
+#include <algorithm>
 #include <limits.h>
 #include <math.h>
-#include <type_traits>
 
 namespace {
 
@@ -49,7 +57,7 @@ struct Args {
     long long ld_allowed;
     const int32_t *state;
     int state_per_row;
-    int units;                       // units per row
+    int run, runs;                   // wide rows: elements of a run, runs of a row
 };
 
 // What a row needs besides its logits.
@@ -61,6 +69,7 @@ template <typename T> struct Row {
     const float *bias;
     const uint32_t *mask;            // null: every token allowed
     bool none;                       // no token allowed
+    __device__ __forceinline__ bool allows(int i) const { return !none && (!mask || ((mask[i >> 5] >> (i & 31)) & 1u)); }
 };
 
 __device__ __forceinline__ float positive(float v) { return v > 0.f && v < __builtin_inff() ? v : __builtin_nanf(""); }
@@ -101,9 +110,11 @@ template <typename T> __device__ __forceinline__ Pack<T> load_pack(const T *p, i
     }
     return v;
 }
+// (Non-temporal: what is written here is read by a later kernel, far more of it than the caches hold.)
+typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(2)));
 template <typename T> __device__ __forceinline__ void store_pack(T *p, const Pack<T> &v, int left) {
     if (left >= Elem<T>::VEC) {
-        *reinterpret_cast<Pack<T> *>(p) = v;
+        __builtin_nontemporal_store(__builtin_bit_cast(Words, v), reinterpret_cast<Words *>(p));
     } else {
 #pragma unroll
         for (int j = 0; j < Elem<T>::VEC; ++j)
@@ -208,402 +219,68 @@ template <int VEC> __device__ __forceinline__ void load_bias(const float *bias, 
     }
 }
 
-// Where a thread stands: which row, which unit, which elements.
-template <typename T, int K, int ROWS> struct Place {
-    static constexpr int VEC = Elem<T>::VEC, THREADS = NT / ROWS, SPAN = THREADS * VEC * K;
-    int r, unit, tid, lane, wave;    // row; unit of the row; thread, lane and wave inside the row's group
-    bool live;
-    __device__ Place(const Args &a, int block) {
-        tid = threadIdx.x & (THREADS - 1), lane = threadIdx.x & 63, wave = ROWS == 1 ? __builtin_amdgcn_readfirstlane(tid >> 6) : 0;
-        if (ROWS == 1) {
-            r = a.units == 1 ? block : (int)((unsigned)block / (unsigned)a.units), unit = block - r * a.units;
-        } else {
-            r = block * ROWS + __builtin_amdgcn_readfirstlane((int)threadIdx.x / THREADS), unit = 0;
-        }
-        live = r < a.R;
-        if (!live) r = a.R - 1;
-    }
-    __device__ __forceinline__ int base() const { return unit * SPAN; }
-    __device__ __forceinline__ int at(int k) const { return ((wave * K + k) * 64 + lane) * VEC; }   // inside the unit
-};
+// a row's token as an element of it, or one that no element is
+__device__ __forceinline__ int token_of(long long tok, int V) { return tok >= 0 && tok < V ? (int)tok : INT_MIN / 2; }
 
-// What the past does to a unit: the count of every id in `cell`, and one bit for every id that occurs in `seen`.
-template <int SPAN> struct Past {
-    int cell[SPAN];
-    uint32_t seen[SPAN / 32];
-};
-struct NoPast {};
-
-// Counts the ids [base, base + n) of the row's history.  Every thread of the workgroup calls it (barriers); the calling group's threads
-// number `tid` of `threads`.
-template <int SPAN>
-__device__ __forceinline__ void count_unit(Past<SPAN> &past, const int64_t *hist, int len, int base, int n, int tid, int threads) {
-    for (int i = tid * 4; i < SPAN; i += threads * 4) *reinterpret_cast<int4 *>(past.cell + i) = make_int4(0, 0, 0, 0);
-    for (int i = tid; i < SPAN / 32; i += threads) past.seen[i] = 0u;
-    __syncthreads();
-#pragma unroll 4
-    for (int j = tid; j < len; j += threads) {
-        const unsigned long long at = (unsigned long long)(hist[j] - base);   // ids outside the vocabulary fall outside every unit
-        if (at < (unsigned long long)n) {
-            atomicAdd(&past.cell[at], 1);
-            atomicOr(&past.seen[at >> 5], 1u << (at & 31));
-        }
-    }
-    __syncthreads();
-}
-
-// A thread's part of a unit: K packs of logits with their bias and mask, requested before the history is walked, and what the walk found.
-//   PAST 0: no history.  1: counts (and bits).  2: `cell` holds the finished value y of every seen id in place of its count, computed
-//   once by one thread; a pack of 64 * VEC ids that has a seen one then costs two instructions an element more, not eight.
-template <typename T, int K, int ROWS, int PAST> struct Unit {
-    using P = Place<T, K, ROWS>;
-    using Lds = std::conditional_t<PAST != 0, Past<P::SPAN>, NoPast>;
-    static constexpr int VEC = P::VEC;
-    P p;
-    Row<T> w;
-    Pack<T> x[K];
-    float b[K][VEC];
-    uint32_t allow[K];               // bit j: element j of the pack is in the row and allowed
-    Lds *past;
-    int n;                           // elements of the unit that the row has
-
-    __device__ __forceinline__ int left(int k) const { return n - p.at(k); }
-    __device__ __forceinline__ int element(int k) const { return p.base() + p.at(k); }
-    __device__ Unit(const Args &a, int block, Lds *lds, bool want_logits) : p(a, block), w(row_of<T>(a, p.r)) {
-        const int base = p.base();
-        n = p.live ? (a.V - base < P::SPAN ? a.V - base : P::SPAN) : 0;
-        past = lds + (ROWS == 1 ? 0 : (int)threadIdx.x / P::THREADS);
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            allow[k] = 0xffffffffu;
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) b[k][j] = 0.f;
-        }
-        if (n == P::SPAN) {          // (no lane's load hangs on a test of its own)
-            if (want_logits) {
-#pragma unroll
-                for (int k = 0; k < K; ++k) x[k] = *reinterpret_cast<const Pack<T> *>(w.x + element(k));
-                if (w.bias) {
-#pragma unroll
-                    for (int k = 0; k < K; ++k) load_bias<VEC>(w.bias + element(k), VEC, b[k]);
-                }
-            }
-            if (w.mask) {
-#pragma unroll
-                for (int k = 0; k < K; ++k) allow[k] = w.mask[element(k) >> 5] >> (element(k) & 31);   // (whole packs: one word)
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-                const int l = left(k);
-                if (want_logits) {
-                    x[k] = load_pack(w.x + element(k), l);
-                    if (w.bias) load_bias<VEC>(w.bias + element(k), l, b[k]);
-                }
-                if (w.mask && l > 0) allow[k] = w.mask[element(k) >> 5] >> (element(k) & 31);
-                allow[k] &= l >= VEC ? 0xffffffffu : l > 0 ? (1u << l) - 1u : 0u;
-            }
-        }
-        if (w.none) {
-#pragma unroll
-            for (int k = 0; k < K; ++k) allow[k] = 0u;
-        }
-        if constexpr (PAST != 0) count_unit(*past, w.hist, p.live ? w.len : 0, base, n, p.tid, P::THREADS);
-    }
-    // PAST 2: one thread for each seen id - the one that takes its bit - leaves y in its cell; the bits are set again as they are taken.
-    __device__ __forceinline__ void finish_seen(const Rule<float> &rule) {
-        for (int i = p.tid; i < P::SPAN / 32; i += P::THREADS) past->seen[i] = 0u;
-        __syncthreads();
-        const int base = p.base(), len = p.live ? w.len : 0;
-#pragma unroll 4
-        for (int j = p.tid; j < len; j += P::THREADS) {
-            const unsigned long long at = (unsigned long long)(w.hist[j] - base);
-            if (at < (unsigned long long)n) {
-                const uint32_t bit = 1u << (at & 31);
-                if (!(atomicOr(&past->seen[at >> 5], bit) & bit)) {
-                    const int i = base + (int)at;
-                    const float v = rule.penalised((float)w.x[i], past->cell[at]) + (w.bias ? w.bias[i] : 0.f);
-                    past->cell[at] = __float_as_int(scaled(v, rule.scale));
-                }
-            }
-        }
-        __syncthreads();
-    }
-    // bit j: element j of pack k has been seen; 0 in every lane unless one of the wave has a bit
-    __device__ __forceinline__ uint32_t seen(int k) const {
-        if constexpr (PAST == 0) return 0u;
-        else return (reinterpret_cast<const uint8_t *>(past->seen)[p.at(k) >> 3] >> (p.at(k) & 7)) & ((1u << VEC) - 1u);
-    }
-    __device__ __forceinline__ void cells(int k, int (&c)[VEC]) const {
-        if constexpr (PAST != 0) {
-#pragma unroll
-            for (int q = 0; q < VEC / 4; ++q) {
-                const int4 v = *reinterpret_cast<const int4 *>(past->cell + p.at(k) + 4 * q);
-                c[4 * q] = v.x, c[4 * q + 1] = v.y, c[4 * q + 2] = v.z, c[4 * q + 3] = v.w;
-            }
-        }
-    }
-    // y of pack k, before the mask
-    __device__ __forceinline__ void values(int k, const Rule<float> &rule, float (&y)[VEC]) const {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) y[j] = scaled((float)x[k].v[j] + b[k][j], rule.scale);
-        if (PAST == 2) {
-            const uint32_t s = seen(k);
-            if (__ballot(s != 0)) {
-                int c[VEC];
-                cells(k, c);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) y[j] = select(bit_word(s, j), __int_as_float(c[j]), y[j]);
-            }
-        }
-    }
-    __device__ __forceinline__ void values(int k, const Rule<double> &rule, double (&y)[VEC]) const {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) y[j] = (double)(float)x[k].v[j];
-        if (PAST == 1) {
-            const uint32_t s = seen(k);
-            if (__ballot(s != 0)) {
-                int c[VEC];
-                cells(k, c);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j)
-                    if (c[j] > 0) y[j] = rule.penalised(y[j], c[j]);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) y[j] = scaled(y[j] + (double)b[k][j], rule.scale);
-    }
-};
-
-template <typename T, int K, int ROWS, bool HIST>
-__global__ __launch_bounds__(NT) void shape_fwd_kernel(Args a, T *__restrict__ out, long long ld_out) {
-    using U = Unit<T, K, ROWS, HIST ? 2 : 0>;
-    __shared__ __align__(16) typename U::Lds lds[ROWS];
-    U u(a, blockIdx.x, lds, true);
-    const Rule<float> rule(u.w, 1.f);
-    if constexpr (HIST) u.finish_seen(rule);
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-        float v[U::VEC];
-        u.values(k, rule, v);
-        Pack<T> y;
-#pragma unroll
-        for (int j = 0; j < U::VEC; ++j) y.v[j] = (T)select(bit_word(u.allow[k], j), v[j], NEG);
-        store_pack(out + u.p.r * ld_out + u.element(k), y, u.left(k));
-    }
-}
-
-// dl = g dy/dl; the logits are read only where the sign of a seen token's decides.
-template <typename T, int K, int ROWS, bool HIST>
-__global__ __launch_bounds__(NT) void shape_bwd_kernel(Args a, const T *__restrict__ g, long long ld_gb, long long ld_gt,
-                                                       T *__restrict__ dx, long long ld_dx) {
-    using U = Unit<T, K, ROWS, HIST ? 1 : 0>;
-    __shared__ __align__(16) typename U::Lds lds[ROWS];
-    U u(a, blockIdx.x, lds, false);
-    const Rule<float> rule(u.w, 1.f);
-    const int b = a.T == 1 ? u.p.r : (int)((unsigned)u.p.r / (unsigned)a.T), t = u.p.r - b * a.T;
-    const T *gr = g + b * ld_gb + t * ld_gt;
-#pragma unroll
-    for (int k = 0; k < K; ++k) u.x[k] = load_pack(gr + u.element(k), u.left(k));
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-        const int i = u.element(k);
-        float v[U::VEC];
-#pragma unroll
-        for (int j = 0; j < U::VEC; ++j) v[j] = (float)u.x[k].v[j] * rule.scale;
-        if (HIST) {
-            const uint32_t s = u.seen(k);
-            if (__ballot(s != 0)) {
-#pragma unroll
-                for (int j = 0; j < U::VEC; ++j)
-                    if ((s >> j) & 1u) v[j] *= rule.factor((float)u.w.x[i + j]);
-            }
-        }
-        Pack<T> d;
-#pragma unroll
-        for (int j = 0; j < U::VEC; ++j) d.v[j] = (T)select(bit_word(u.allow[k], j), v[j], 0.f);
-        store_pack(dx + u.p.r * ld_dx + i, d, u.left(k));
-    }
-}
-
+// exp(y - m) as a power of two.  (The difference first: a row of the type's lowest values - masked by hand - has an m whose multiple of
+// log2 e overflows.)  Where nothing is allowed m = -inf: 0 in its place.
+constexpr float LOG2E = 1.4426950408889634f;
+__device__ __forceinline__ float reference_of(float m) { return m == NEG ? 0.f : m; }
+__device__ __forceinline__ float exp_from(float y, float from) { return __builtin_amdgcn_exp2f((y - from) * LOG2E); }
 __device__ __forceinline__ float log_prob_of(float y_tok, float m, float s) {
     return m == NEG && s == 0.f ? NEG : y_tok - m - logf(s);   // (nothing allowed: log 0)
 }
 
-// a row's token as an element of it, or one that no pack holds
-__device__ __forceinline__ int token_of(long long tok, int V) { return tok >= 0 && tok < V ? (int)tok : INT_MIN / 2; }
-
-// exp(y - m) as a power of two.  (The difference first: a row of the type's lowest values - masked by hand - has an m whose multiple of
-// log2 e overflows.)  A piece that allows nothing has m = -inf: 0 in its place.
-constexpr float LOG2E = 1.4426950408889634f;
-__device__ __forceinline__ float reference_of(float m) { return m == NEG ? 0.f : m; }
-__device__ __forceinline__ float exp_from(float y, float m) { return __builtin_amdgcn_exp2f((y - m) * LOG2E); }
-
-// Per wave: the maximum and the sum of exponentials of its piece; per row: the shaped value of its token.  ROWS > 1: the wave has the
-// whole row and finishes it.  Sums are 32-bit: 64 lanes of at most VEC * K terms each, then 6 levels, so the relative error stays below
-// (VEC * K + 6 + pieces) * 2^-24.
-template <typename T, int K, int ROWS, bool HIST>
-__global__ __launch_bounds__(NT) void log_prob_fwd_kernel(Args a, const int64_t *__restrict__ tokens, float *__restrict__ lp,
-                                                          float2 *__restrict__ stats, float2 *__restrict__ part,
-                                                          float *__restrict__ target) {
-    using U = Unit<T, K, ROWS, HIST ? 2 : 0>;
-    __shared__ __align__(16) typename U::Lds lds[ROWS];
-    U u(a, blockIdx.x, lds, true);
-    const Rule<float> rule(u.w, 1.f);
-    if constexpr (HIST) u.finish_seen(rule);
-    if (!u.p.live) return;
-    const int tok = token_of(tokens[u.p.r], a.V);
-    float y[K][U::VEC];
-    float m = NEG, yt = 0.f;
-    bool mine = false;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-        u.values(k, rule, y[k]);
-#pragma unroll
-        for (int j = 0; j < U::VEC; ++j) {
-            y[k][j] = select(bit_word(u.allow[k], j), y[k][j], NEG);
-            m = fmaxf(m, y[k][j]);
-        }
-        const unsigned at = (unsigned)(tok - u.element(k));
-        if (at < (unsigned)U::VEC) {
-            mine = true;
-#pragma unroll
-            for (int j = 0; j < U::VEC; ++j)
-                if (j == (int)at) yt = y[k][j];
-        }
-    }
-    m = wave_max(m);
-    const float from = reference_of(m);
-    float s = 0.f;
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int j = 0; j < U::VEC; ++j) s += exp_from(y[k][j], from);
-    s = wave_sum(s);
-    if (ROWS == 1) {
-        if (mine) target[u.p.r] = yt;
-        if (u.p.lane == 0) part[(long long)u.p.r * a.units * WAVES + u.p.unit * WAVES + u.p.wave] = make_float2(m, s);
-        return;
-    }
-    const unsigned long long owner = __ballot(mine);
-    const float v = owner ? log_prob_of(from_lane(yt, __ffsll((long long)owner) - 1), m, s) : 0.f;
-    if (u.p.lane == 0) lp[u.p.r] = v, stats[u.p.r] = make_float2(m, s);
-}
-
-// One wave per row: the pieces' maxima and sums joined.
-__global__ __launch_bounds__(NT) void log_prob_join_kernel(int R, int V, int pieces, const int64_t *__restrict__ tokens,
-                                                           const float2 *__restrict__ part, const float *__restrict__ target,
-                                                           float *__restrict__ lp, float2 *__restrict__ stats) {
-    const int lane = threadIdx.x & 63, r = blockIdx.x * WAVES + (threadIdx.x >> 6);
-    if (r >= R) return;
-    const float2 *p = part + (long long)r * pieces;
-    float m = NEG;
-    for (int i = lane; i < pieces; i += 64) m = fmaxf(m, p[i].x);
-    m = wave_max(m);
-    float s = 0.f;
-    for (int i = lane; i < pieces; i += 64) {
-        const float2 q = p[i];
-        s += q.x == NEG ? q.y : q.y * __expf(q.x - m);   // (an empty piece adds its 0, one that holds nothing but NaN its NaN)
-    }
-    s = wave_sum(s);
-    if (lane != 0) return;
-    const long long tok = tokens[r];
-    lp[r] = tok >= 0 && tok < V ? log_prob_of(target[r], m, s) : 0.f;
-    stats[r] = make_float2(m, s);
-}
-
-template <typename T, int K, int ROWS, bool HIST>
-__global__ __launch_bounds__(NT) void log_prob_bwd_kernel(Args a, const int64_t *__restrict__ tokens, const float2 *__restrict__ stats,
-                                                          const float *__restrict__ g, T *__restrict__ dx, long long ld_dx) {
-    using U = Unit<T, K, ROWS, HIST ? 2 : 0>;
-    __shared__ __align__(16) typename U::Lds lds[ROWS];
-    U u(a, blockIdx.x, lds, true);
-    const Rule<float> rule(u.w, 1.f);
-    if constexpr (HIST) u.finish_seen(rule);
-    const int tok = token_of(tokens[u.p.r], a.V);
-    const float2 st = stats[u.p.r];
-    const bool zero = tok < 0 || (st.x == NEG && st.y == 0.f);   // a row without a token, or with none allowed
-    const float at_token = g[u.p.r] * rule.scale, others = -at_token / st.y, from = reference_of(st.x);
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-        const int i = u.element(k);
-        float v[U::VEC];
-        u.values(k, rule, v);
-#pragma unroll
-        for (int j = 0; j < U::VEC; ++j) v[j] = others * exp_from(v[j], from);
-        const unsigned at = (unsigned)(tok - i);
-        if (at < (unsigned)U::VEC) {
-#pragma unroll
-            for (int j = 0; j < U::VEC; ++j)
-                if (j == (int)at) v[j] += at_token;
-        }
-        if (HIST) {
-            const uint32_t s = u.seen(k);
-            if (__ballot(s != 0)) {
-#pragma unroll
-                for (int j = 0; j < U::VEC; ++j) v[j] = select(bit_word(s, j), v[j] * rule.factor((float)u.x[k].v[j]), v[j]);
-            }
-        }
-        const uint32_t bits = zero ? 0u : u.allow[k];
-        Pack<T> d;
-#pragma unroll
-        for (int j = 0; j < U::VEC; ++j) d.v[j] = (T)select(bit_word(bits, j), v[j], 0.f);
-        store_pack(dx + u.p.r * ld_dx + i, d, u.left(k));
-    }
-}
-
-// ---- draw.  The pick is a decision: with a running sum in 32 bits, u * total falls on the wrong side of some boundary about once in
-// 1e3 .. 1e4 rows at V = 1e5 (V boundaries, each off by ~1e-8), and differently for every tiling.  So values, exponentials and sums are
-// 64-bit here: the pick is the one of the exact distribution but for ~1e-9 of the rows, whatever the tiling.
-struct Piece {
-    double s, m;                     // sum of 2^(z - m), largest z;  z = y log2 e
-};
+// ---- 64-bit arithmetic of the draw.  The pick is a decision: with a running sum in 32 bits, u * total falls on the wrong side of some
+// boundary about once in 1e3 .. 1e4 rows at V = 1e5 (V boundaries, each off by ~1e-8), and differently for every tiling.  So values,
+// exponentials and sums are 64-bit: the pick is the one of the exact distribution but for ~1e-8 of the rows, whatever the tiling.
 constexpr double NEG64 = -__builtin_inf(), LOG2E64 = 1.4426950408889634;
 
-// 2^z for z <= 0 (0 below 2^-1074): 2^n of the nearest whole number times the series of 2^r = e^(r ln 2), |r| <= 1/2, whose rest after
-// the 11th power is below 7e-15 of the value.
+// 2^z for z <= 0 (0 below 2^-1074): 2^n of the nearest whole number times a polynomial in the rest |r| <= 1/2 - the one of degree 9 that is 1
+// at r = 0 and has the smallest largest relative error (Remez exchange: 7.7e-14).
 __device__ __forceinline__ double power_of_two(double z) {
     z = fmax(z, -1080.);
     const double n = rint(z), r = z - n;
-    double p = 4.4455382718708116e-10;
-    p = fma(p, r, 7.054911620801123e-09);
-    p = fma(p, r, 1.01780860092397e-07);
-    p = fma(p, r, 1.321548679014431e-06);
-    p = fma(p, r, 1.5252733804059841e-05);
-    p = fma(p, r, 0.0001540353039338161);
-    p = fma(p, r, 0.0013333558146428443);
-    p = fma(p, r, 0.009618129107628477);
-    p = fma(p, r, 0.05550410866482158);
-    p = fma(p, r, 0.24022650695910072);
-    p = fma(p, r, 0.6931471805599453);
+    double p = 9.16811938851594e-08;
+    p = fma(p, r, 1.3255182784592006e-06);
+    p = fma(p, r, 1.5258493063907014e-05);
+    p = fma(p, r, 0.0001540345603665657);
+    p = fma(p, r, 0.0013333547331461978);
+    p = fma(p, r, 0.009618129159172244);
+    p = fma(p, r, 0.055504108739712246);
+    p = fma(p, r, 0.24022650695813708);
+    p = fma(p, r, 0.6931471805585505);
     p = fma(p, r, 1.);
     return ldexp(p, (int)n);
 }
 
-// e[k][j] = 2^(z - m) of the thread's elements (0 where not allowed), m the wave's largest z, which is returned: NaN if a value that is
-// allowed is NaN.
-template <typename T, int K, int ROWS, int PAST, int VEC>
-__device__ __forceinline__ double exp_values(const Unit<T, K, ROWS, PAST> &u, double (&e)[K][VEC]) {
-    const Rule<double> rule(u.w, LOG2E64);
-    double m = NEG64;
-    bool bad = false;
+// The reference m of a wave's z (log2 e times y; -inf where not allowed) from each lane's largest: near or at the largest of all.
+__device__ __forceinline__ double reference_of(double top) {
+    // a 32-bit maximum serves while its rounding is small in z's units
+    const double m = (double)wave_max((float)top);
+    return fabs(m) < 1e6 ? m : wave_max(top);
+}
+template <int K, int VEC> __device__ __forceinline__ void largest(const double (&z)[K][VEC], double &top, bool &bad) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        u.values(k, rule, e[k]);
+    for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            e[k][j] = select(bit_word(u.allow[k], j), e[k][j], NEG64);
-            bad |= e[k][j] != e[k][j];
-            m = fmax(m, e[k][j]);
-        }
-    }
-    m = wave_max(m);
+        for (int j = 0; j < VEC; ++j) bad |= z[k][j] != z[k][j], top = fmax(top, z[k][j]);
+}
+// z becomes 2^(z - m), 0 where not allowed
+template <int K, int VEC> __device__ __forceinline__ void exponentials(double (&z)[K][VEC], double m) {
     const double from = m == NEG64 ? 0. : m;
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) e[k][j] = power_of_two(e[k][j] - from);
-    return __ballot(bad) ? __builtin_nan("") : m;
+        for (int j = 0; j < VEC; ++j) z[k][j] = power_of_two(z[k][j] - from);
+}
+template <int K, int VEC> __device__ __forceinline__ double lane_sum(const double (&e)[K][VEC]) {
+    double s = 0.;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) s += e[k][j];
+    return s;
 }
 
 // The first element, in index order, at which the running sum (starting from `before`) exceeds thr; the last positive one if it never
@@ -638,69 +315,664 @@ template <int K, int VEC> __device__ __forceinline__ Pick pick_in_wave(const dou
     }
     return found;
 }
-
 __device__ __forceinline__ float draw_log_prob(double value, double total) { return (float)log(value / total); }
 
-// a whole row in a wave
-template <typename T, int K, int ROWS, bool HIST>
-__global__ __launch_bounds__(NT) void draw_row_kernel(Args a, const float *__restrict__ uniforms, long long ld_u, int64_t empty,
-                                                      int64_t *__restrict__ out, float *__restrict__ lp) {
-    using U = Unit<T, K, ROWS, HIST ? 1 : 0>;
-    __shared__ __align__(16) typename U::Lds lds[ROWS];
-    U u(a, blockIdx.x, lds, true);
-    if (!u.p.live) return;
-    double e[K][U::VEC];
-    const double m = exp_values(u, e);
-    double s = 0.;
+// ---- packs: K of them are a thread's share of 64 * VEC * K neighbouring elements, pack k holding elements (k * 64 + lane) * VEC of these.
+template <typename T, int K, bool BIAS> struct Packs {
+    static constexpr int VEC = Elem<T>::VEC, SPAN = 64 * VEC * K;
+    Pack<T> x[K];                    // logits (or what `from` holds)
+    float b[BIAS ? K : 1][VEC];
+    uint32_t allow[K];               // bit j: element j of the pack is in the row and allowed
+    static __device__ __forceinline__ int at(int k) { return (k * 64 + ((int)threadIdx.x & 63)) * VEC; }
+
+    // Elements [base, base + SPAN) of a row, all inside it.  The same loads in every lane and on every path, so that the wait for these packs
+    // can leave the next ones in flight: without a mask the word loaded is any word, and is overruled.
+    __device__ __forceinline__ void load(const T *from, const Row<T> &w, int base) {
+        // (an address in global memory for certain: a load that might be from LDS would be waited for with LDS's own)
+        typedef const __attribute__((address_space(1))) uint32_t *Global;
+        const Global mask = (Global)(w.mask ? (uintptr_t)w.mask : (uintptr_t)w.x & ~(uintptr_t)3);   // (the 4 bytes that hold the first logit)
+        const int which = w.mask ? ~0 : 0;
+        const uint32_t all = w.mask ? 0u : 0xffffffffu;
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+        for (int k = 0; k < K; ++k) x[k] = *reinterpret_cast<const Pack<T> *>(from + base + at(k));
+        if constexpr (BIAS) {
 #pragma unroll
-        for (int j = 0; j < U::VEC; ++j) s += e[k][j];
-    s = wave_sum(s);
-    const Pick pick = pick_in_wave(e, 0., (double)uniforms[u.p.r * ld_u] * s);
-    if (u.p.lane == 0) {
-        const bool ok = s > 0. && m < __builtin_inf() && pick.index >= 0;
-        out[u.p.r] = ok ? pick.index : empty;
-        lp[u.p.r] = ok ? draw_log_prob(pick.value, s) : (m == NEG64 ? NEG : __builtin_nanf(""));
+            for (int k = 0; k < K; ++k) load_bias<VEC>(w.bias + base + at(k), VEC, b[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int i = base + at(k);                      // (whole packs: their bits are in one word)
+            allow[k] = ((mask[(i >> 5) & which] >> (i & 31)) | all) & (w.none ? 0u : 0xffffffffu);
+        }
+    }
+    // The same for a row's end: elements of [base, V).
+    __device__ __forceinline__ void load_end(const T *from, const Row<T> &w, int base, int V) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int i = base + at(k), left = V - i;
+            x[k] = load_pack(from + i, left);
+            if constexpr (BIAS) load_bias<VEC>(w.bias + i, left, b[k]);
+            allow[k] = left >= VEC ? 0xffffffffu : left > 0 ? (1u << left) - 1u : 0u;
+            if (w.mask && left > 0) allow[k] &= w.mask[i >> 5] >> (i & 31);
+            if (w.none) allow[k] = 0u;
+        }
+    }
+    // y as if nothing had been seen, before the mask
+    template <typename C> __device__ __forceinline__ void raw(int k, const Rule<C> &rule, C (&y)[VEC]) const {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            y[j] = (C)(float)x[k].v[j];
+            if constexpr (BIAS) y[j] += (C)b[k][j];
+            y[j] = scaled(y[j], rule.scale);
+        }
+    }
+    template <typename C> __device__ __forceinline__ void masked(int k, C no, C (&y)[VEC]) const {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) y[j] = select(bit_word(allow[k], j), y[j], no);
+    }
+};
+template <typename T, int VEC> __device__ __forceinline__ Pack<T> rounded(const float (&v)[VEC]) {
+    Pack<T> p;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) p.v[j] = (T)v[j];
+    return p;
+}
+
+// ---- rows of at most ROW_MAX elements: a wave each.  The counts of all ids are a dense array.
+constexpr int ROW_MAX = 1024;
+template <int SPAN> struct Counts {
+    int cell[SPAN];
+};
+
+template <typename T, int K, bool BIAS> struct Narrow {
+    using P = Packs<T, K, BIAS>;
+    using Lds = Counts<P::SPAN>;
+    static constexpr int VEC = P::VEC;
+    int r, lane;
+    bool live, past;
+    Row<T> w;
+    P p;
+    Lds *lds;
+    __device__ Narrow(const Args &a, Lds *all, const T *from, long long ld_b, long long ld_t) {
+        const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+        lane = threadIdx.x & 63, r = blockIdx.x * WAVES + wave, live = r < a.R, past = a.history != nullptr, lds = all + wave;
+        if (!live) r = a.R - 1;      // (such a wave only keeps the barriers company)
+        w = row_of<T>(a, r);
+        const int b = a.T == 1 ? r : (int)((unsigned)r / (unsigned)a.T), t = r - b * a.T;
+        p.load_end(from + b * ld_b + t * ld_t, w, 0, a.V);
+        if (past) {
+            for (int i = lane * 4; i < P::SPAN; i += 256) *reinterpret_cast<int4 *>(lds->cell + i) = make_int4(0, 0, 0, 0);
+            __syncthreads();
+#pragma unroll 4
+            for (int j = lane; j < w.len; j += 64) {
+                const unsigned long long id = (unsigned long long)w.hist[j];
+                if (id < (unsigned long long)a.V) atomicAdd(&lds->cell[id], 1);
+            }
+            __syncthreads();
+        }
+    }
+    // the counts of pack k; whether any lane of the wave has one above 0
+    __device__ __forceinline__ bool counts(int k, int (&c)[VEC]) const {
+        if (!past) return false;
+        int any = 0;
+#pragma unroll
+        for (int q = 0; q < VEC / 4; ++q) {
+            const int4 v = *reinterpret_cast<const int4 *>(lds->cell + P::at(k) + 4 * q);
+            c[4 * q] = v.x, c[4 * q + 1] = v.y, c[4 * q + 2] = v.z, c[4 * q + 3] = v.w;
+            any |= (v.x | v.y) | (v.z | v.w);
+        }
+        return __ballot(any != 0) != 0;
+    }
+    // y of pack k, before the mask
+    template <typename C> __device__ __forceinline__ void values(int k, const Rule<C> &rule, C (&y)[VEC]) const {
+        int c[VEC];
+        if (counts(k, c)) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const C x = (C)(float)p.x[k].v[j];
+                y[j] = c[j] > 0 ? rule.penalised(x, c[j]) : x;
+                if constexpr (BIAS) y[j] += (C)p.b[k][j];
+                y[j] = scaled(y[j], rule.scale);
+            }
+        } else {
+            p.raw(k, rule, y);
+        }
+    }
+};
+
+// ---- wider rows: runs
+// What a run's workgroup knows of the row's past.  bits: one for each element of the run; the list of the seen ones in the order of the
+// bits, entry rank[i / 32] being the first of word i / 32: id (the element of the run) and its finished value, -inf where the mask forbids it.
+template <typename C> struct Seen {
+    C *value;
+    uint32_t *bits;
+    uint16_t *rank, *id;
+    int total;                       // entries of the list
+    static size_t bytes(int run, int len) {
+        const int cap = len < run ? len : run;
+        return ((size_t)cap * (sizeof(C) + 2) + 15) / 16 * 16 + (size_t)run / 32 * 6;
+    }
+    __device__ Seen(char *lds, int run, int len) : total(0) {
+        const int cap = len < run ? len : run;
+        value = reinterpret_cast<C *>(lds), id = reinterpret_cast<uint16_t *>(lds + (size_t)cap * sizeof(C));
+        bits = reinterpret_cast<uint32_t *>(lds + ((size_t)cap * (sizeof(C) + 2) + 15) / 16 * 16);
+        rank = reinterpret_cast<uint16_t *>(bits + run / 32);
+    }
+};
+
+constexpr int RUN_MAX = 32768;       // ranks and ids fit 16 bits; 1024 words of bits, 4 for each thread
+constexpr int HELD = 4;              // ids of the history that a thread keeps between the walks
+
+// One walk over the row's history: f(element of the run) for every id in it.
+template <typename F> __device__ __forceinline__ void walk(const int (&held)[HELD], const int64_t *hist, int len, int base, int n, F f) {
+#pragma unroll
+    for (int q = 0; q < HELD; ++q)
+        if (held[q] >= 0) f(held[q]);
+#pragma unroll 4
+    for (int j = HELD * NT + threadIdx.x; j < len; j += NT) {
+        const unsigned long long at = (unsigned long long)(hist[j] - base);   // ids outside the vocabulary fall outside every run
+        if (at < (unsigned long long)n) f((int)at);
     }
 }
 
-template <typename T, int K, bool HIST>
-__global__ __launch_bounds__(NT) void draw_piece_kernel(Args a, Piece *__restrict__ part) {
-    using U = Unit<T, K, 1, HIST ? 1 : 0>;
-    __shared__ __align__(16) typename U::Lds lds[1];
-    U u(a, blockIdx.x, lds, true);
-    double e[K][U::VEC];
-    const double m = exp_values(u, e);
-    double s = 0.;
+// Sets the bits of the seen elements of [base, base + n); with LIST also ranks and the list of finished values.  The workgroup calls it.
+template <bool LIST, typename T, typename C>
+__device__ __forceinline__ void look_back(Seen<C> &seen, const Row<T> &w, const Rule<C> &rule, int base, int n) {
+    __shared__ int wave_total[WAVES];
+    const int words = (n + 31) >> 5, tid = threadIdx.x;
+    int held[HELD];
+#pragma unroll
+    for (int q = 0; q < HELD; ++q) {
+        held[q] = -1;
+        if (tid + q * NT < w.len) {
+            const unsigned long long at = (unsigned long long)(w.hist[tid + q * NT] - base);
+            if (at < (unsigned long long)n) held[q] = (int)at;
+        }
+    }
+    for (int i = tid; i < words; i += NT) seen.bits[i] = 0u;
+    __syncthreads();
+    walk(held, w.hist, w.len, base, n, [&](int at) { atomicOr(&seen.bits[at >> 5], 1u << (at & 31)); });
+    __syncthreads();
+    if constexpr (LIST) {
+        // ranks: every thread 4 words, their bits counted and summed over the workgroup
+        int here[RUN_MAX / 32 / NT], mine = 0;
+#pragma unroll
+        for (int q = 0; q < RUN_MAX / 32 / NT; ++q) {
+            const int i = tid * (RUN_MAX / 32 / NT) + q;
+            here[q] = mine;
+            mine += i < words ? __popc(seen.bits[i]) : 0;
+        }
+        const int upto = (int)wave_scan((float)mine);   // (exact: at most 32768)
+        if ((tid & 63) == 63) wave_total[tid >> 6] = upto;
+        __syncthreads();
+        int first = upto - mine, total = 0;
+#pragma unroll
+        for (int v = 0; v < WAVES; ++v) {
+            if (v < (tid >> 6)) first += wave_total[v];
+            total += wave_total[v];
+        }
+        seen.total = total;
+#pragma unroll
+        for (int q = 0; q < RUN_MAX / 32 / NT; ++q) {
+            const int i = tid * (RUN_MAX / 32 / NT) + q;
+            if (i < words) seen.rank[i] = (uint16_t)(first + here[q]);
+        }
+        int *count = reinterpret_cast<int *>(seen.value);   // cell u of the list: first its count, in the cell's first 4 bytes
+        constexpr int STEP = sizeof(C) / 4;
+        for (int u = tid; u < total; u += NT) count[u * STEP] = 0;
+        __syncthreads();
+        walk(held, w.hist, w.len, base, n, [&](int at) {
+            const uint32_t word = seen.bits[at >> 5];
+            const int u = seen.rank[at >> 5] + __popc(word & ((1u << (at & 31)) - 1u));
+            atomicAdd(&count[u * STEP], 1);
+            seen.id[u] = (uint16_t)at;                       // (the same from every thread that holds the id)
+        });
+        __syncthreads();
+        for (int u = tid; u < total; u += NT) {
+            const int at = seen.id[u], i = base + at;
+            const C v = rule.penalised((C)(float)w.x[i], count[u * STEP]) + (w.bias ? (C)w.bias[i] : (C)0);
+            seen.value[u] = w.allows(i) ? scaled(v, rule.scale) : (C)NEG;
+        }
+        __syncthreads();
+    }
+}
+
+// Where a workgroup's run lies.
+struct Place {
+    int r, base, n;
+    __device__ Place(const Args &a, int block) {
+        r = a.runs == 1 ? block : (int)((unsigned)block / (unsigned)a.runs);
+        base = (block - r * a.runs) * a.run;
+        n = a.V - base < a.run ? a.V - base : a.run;
+    }
+};
+
+// bits of the seen elements of the pack that begins at element `at` of the run
+template <int VEC, typename C> __device__ __forceinline__ uint32_t seen_bits(const Seen<C> &seen, int at, int n) {
+    return at < n ? (seen.bits[at >> 5] >> (at & 31)) & ((1u << VEC) - 1u) : 0u;
+}
+// Streams through a run: `f(packs, element of the row that they begin at)` for every step of SPAN elements, the steps shared out to the
+// waves in turn; a step's loads are requested while the step before is worked on, the first before `prepare()` runs.
+template <typename P, typename T, typename Prepare, typename F>
+__device__ __forceinline__ void stream(const Args &a, const Place &at, const Row<T> &w, const T *from, Prepare prepare, F f) {
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), full = at.n / P::SPAN;
+    P one, two;
+    int s = wave;
+    if (s < full) one.load(from, w, at.base + s * P::SPAN);
+    prepare();
+    if (s < full) {
+        const int last = full - 1 - ((full - 1 - wave) & (WAVES - 1));   // (after the last step it is requested once more: no path without loads)
+        for (;;) {
+            two.load(from, w, at.base + std::min(s + WAVES, last) * P::SPAN);
+            f(one, at.base + s * P::SPAN);
+            s += WAVES;
+            if (s >= full) break;
+            one.load(from, w, at.base + std::min(s + WAVES, last) * P::SPAN);
+            f(two, at.base + s * P::SPAN);
+            s += WAVES;
+            if (s >= full) break;
+        }
+    }
+    if (s == full && full * P::SPAN < at.n) {
+        one.load_end(from, w, at.base + s * P::SPAN, a.V);
+        f(one, at.base + s * P::SPAN);
+    }
+}
+
+extern __shared__ __align__(16) char run_lds[];
+
+// ---- shape
+template <typename T, int K, bool BIAS>
+__global__ __launch_bounds__(NT) void shape_rows_kernel(Args a, T *__restrict__ out, long long ld_out) {
+    using N = Narrow<T, K, BIAS>;
+    __shared__ __align__(16) typename N::Lds lds[WAVES];
+    N u(a, lds, (const T *)a.logits, a.ld_b, a.ld_t);
+    if (!u.live) return;
+    const Rule<float> rule(u.w, 1.f);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        float v[N::VEC];
+        u.values(k, rule, v);
+        u.p.masked(k, NEG, v);
+        store_pack(out + u.r * ld_out + N::P::at(k), rounded<T>(v), a.V - N::P::at(k));
+    }
+}
+
+template <typename T, int K, bool BIAS> __global__ __launch_bounds__(NT) void shape_run_kernel(Args a, T *__restrict__ out, long long ld_out) {
+    using P = Packs<T, K, BIAS>;
+    const Place at(a, blockIdx.x);
+    const Row<T> w = row_of<T>(a, at.r);
+    const Rule<float> rule(w, 1.f);
+    Seen<float> seen(run_lds, a.run, a.L);
+    T *row = out + at.r * ld_out;
+    stream<P>(a, at, w, w.x, [&] { if (a.history) look_back<true>(seen, w, rule, at.base, at.n); },
+                 [&](const P &p, int first) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int i = first + P::at(k);
+            float v[P::VEC];
+            p.raw(k, rule, v);
+            p.masked(k, NEG, v);
+            store_pack(row + i, rounded<T>(v), a.V - i);
+        }
+    });
+    if (a.history) {
+        __syncthreads();             // (orders these stores after the stream's)
+        for (int u = threadIdx.x; u < seen.total; u += NT) row[at.base + seen.id[u]] = (T)seen.value[u];
+    }
+}
+
+// dl = g dy/dl; the logits are read only where the sign of a seen token's decides.
+template <typename T, int K>
+__global__ __launch_bounds__(NT) void shape_rows_bwd_kernel(Args a, const T *__restrict__ g, long long ld_gb, long long ld_gt,
+                                                            T *__restrict__ dx, long long ld_dx) {
+    using N = Narrow<T, K, false>;
+    __shared__ __align__(16) typename N::Lds lds[WAVES];
+    N u(a, lds, g, ld_gb, ld_gt);
+    if (!u.live) return;
+    const Rule<float> rule(u.w, 1.f);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        float v[N::VEC];
+        u.p.raw(k, rule, v);
+        int c[N::VEC];
+        if (u.counts(k, c)) {
+#pragma unroll
+            for (int j = 0; j < N::VEC; ++j)
+                if (c[j] > 0) v[j] *= rule.factor((float)u.w.x[N::P::at(k) + j]);
+        }
+        u.p.masked(k, 0.f, v);
+        store_pack(dx + u.r * ld_dx + N::P::at(k), rounded<T>(v), a.V - N::P::at(k));
+    }
+}
+
+template <typename T, int K>
+__global__ __launch_bounds__(NT) void shape_run_bwd_kernel(Args a, const T *__restrict__ g, long long ld_gb, long long ld_gt,
+                                                           T *__restrict__ dx, long long ld_dx) {
+    using P = Packs<T, K, false>;
+    const Place at(a, blockIdx.x);
+    const Row<T> w = row_of<T>(a, at.r);
+    const Rule<float> rule(w, 1.f);
+    Seen<float> seen(run_lds, a.run, 0);                 // (bits alone)
+    const int b = a.T == 1 ? at.r : (int)((unsigned)at.r / (unsigned)a.T), t = at.r - b * a.T;
+    stream<P>(a, at, w, g + b * ld_gb + t * ld_gt, [&] { if (a.history) look_back<false>(seen, w, rule, at.base, at.n); },
+                 [&](const P &p, int first) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int i = first + P::at(k);
+            float v[P::VEC];
+            p.raw(k, rule, v);
+            if (a.history) {
+                const uint32_t s = seen_bits<P::VEC>(seen, i - at.base, at.n);
+                if (s) {
+#pragma unroll
+                    for (int j = 0; j < P::VEC; ++j)
+                        if ((s >> j) & 1u) v[j] *= rule.factor((float)w.x[i + j]);
+                }
+            }
+            p.masked(k, 0.f, v);
+            store_pack(dx + at.r * ld_dx + i, rounded<T>(v), a.V - i);
+        }
+    });
+}
+
+// ---- log_prob.  Sums are 32-bit: a lane's at most 128 terms of a run in a chain (rescaled where its maximum grows), 6 levels over
+// the wave, 4 waves, then the row's runs: the relative error stays below (128 + 10 + runs) * 2^-24 and is far below it on average.
+template <typename T, int K, bool BIAS>
+__global__ __launch_bounds__(NT) void log_prob_rows_kernel(Args a, const int64_t *__restrict__ tokens, float *__restrict__ lp,
+                                                           float2 *__restrict__ stats) {
+    using N = Narrow<T, K, BIAS>;
+    __shared__ __align__(16) typename N::Lds lds[WAVES];
+    N u(a, lds, (const T *)a.logits, a.ld_b, a.ld_t);
+    if (!u.live) return;
+    const Rule<float> rule(u.w, 1.f);
+    const int tok = token_of(tokens[u.r], a.V);
+    float y[K][N::VEC], m = NEG, yt = 0.f;
+    bool mine = false;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        u.values(k, rule, y[k]);
+        u.p.masked(k, NEG, y[k]);
+#pragma unroll
+        for (int j = 0; j < N::VEC; ++j) {
+            m = fmaxf(m, y[k][j]);
+            if (tok == N::P::at(k) + j) yt = y[k][j], mine = true;
+        }
+    }
+    m = wave_max(m);
+    const float from = reference_of(m);
+    float s = 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int j = 0; j < U::VEC; ++j) s += e[k][j];
+        for (int j = 0; j < N::VEC; ++j) s += exp_from(y[k][j], from);
     s = wave_sum(s);
-    if (u.p.lane == 0) part[(long long)u.p.r * a.units * WAVES + u.p.unit * WAVES + u.p.wave] = Piece{s, m};
+    const unsigned long long owner = __ballot(mine);
+    const float v = owner ? log_prob_of(from_lane(yt, __ffsll((long long)owner) - 1), m, s) : 0.f;
+    if (u.lane == 0) lp[u.r] = v, stats[u.r] = make_float2(m, s);
 }
 
-// One workgroup per row: the pieces joined in index order, the piece that holds u * total found, and its elements computed and walked
-// again, a slab of it for each wave.
-template <typename T, int K, bool HIST>
+// (maximum, sum) pairs joined: the sums in units of the common maximum.  An empty part adds its 0, one that holds nothing but NaN its NaN.
+__device__ __forceinline__ float rebased(float2 part, float m) { return part.x == NEG ? part.y : part.y * exp_from(part.x, reference_of(m)); }
+
+template <typename T, int K, bool BIAS>
+__global__ __launch_bounds__(NT) void log_prob_run_kernel(Args a, const int64_t *__restrict__ tokens, float *__restrict__ lp,
+                                                          float2 *__restrict__ stats, float2 *__restrict__ part, float *__restrict__ target) {
+    using P = Packs<T, K, BIAS>;
+    __shared__ float2 waves[WAVES];
+    __shared__ float at_token;
+    const Place at(a, blockIdx.x);
+    const Row<T> w = row_of<T>(a, at.r);
+    const Rule<float> rule(w, 1.f);
+    Seen<float> seen(run_lds, a.run, a.L);
+    const int tok = token_of(tokens[at.r], a.V);
+    float m = NEG, s = 0.f;          // of this lane's elements so far
+    stream<P>(a, at, w, w.x, [&] { if (a.history) look_back<true>(seen, w, rule, at.base, at.n); },
+                 [&](const P &p, int first) {
+        float y[K][P::VEC], top = m;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int i = first + P::at(k);
+            p.raw(k, rule, y[k]);
+            uint32_t left_out = 0u;
+            if (a.history) left_out = seen_bits<P::VEC>(seen, i - at.base, at.n);
+            const uint32_t allow = p.allow[k] & ~left_out;
+#pragma unroll
+            for (int j = 0; j < P::VEC; ++j) y[k][j] = select(bit_word(allow, j), y[k][j], NEG), top = fmaxf(top, y[k][j]);
+            const unsigned here = (unsigned)(tok - i);
+            if (here < (unsigned)P::VEC && !((left_out >> here) & 1u)) {
+#pragma unroll
+                for (int j = 0; j < P::VEC; ++j)
+                    if (j == (int)here) at_token = y[k][j];
+            }
+        }
+        const float from = reference_of(top);
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int j = 0; j < P::VEC; ++j) sum += exp_from(y[k][j], from);
+        s = s * exp_from(m, from) + sum, m = top;
+    });
+    if (a.history) {
+        for (int u = threadIdx.x; u < seen.total; u += NT) {
+            const float y = seen.value[u], top = fmaxf(m, y), from = reference_of(top);
+            s = s * exp_from(m, from) + exp_from(y, from), m = top;
+            if (at.base + seen.id[u] == tok) at_token = y;
+        }
+    }
+    const float top = wave_max(m);
+    s = wave_sum(rebased(make_float2(m, s), top));
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = make_float2(top, s);
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    m = NEG, s = 0.f;
+    for (int v = 0; v < WAVES; ++v) m = fmaxf(m, waves[v].x);
+    for (int v = 0; v < WAVES; ++v) s += rebased(waves[v], m);
+    if (a.runs == 1) {
+        lp[at.r] = tok >= 0 ? log_prob_of(at_token, m, s) : 0.f, stats[at.r] = make_float2(m, s);
+    } else {
+        part[(long long)at.r * a.runs + at.base / a.run] = make_float2(m, s);
+        if (tok >= at.base && tok < at.base + at.n) target[at.r] = at_token;
+    }
+}
+
+// One wave per row: its runs joined.
+__global__ __launch_bounds__(NT) void log_prob_join_kernel(int R, int V, int runs, const int64_t *__restrict__ tokens,
+                                                           const float2 *__restrict__ part, const float *__restrict__ target,
+                                                           float *__restrict__ lp, float2 *__restrict__ stats) {
+    const int lane = threadIdx.x & 63, r = blockIdx.x * WAVES + (threadIdx.x >> 6);
+    if (r >= R) return;
+    const float2 *p = part + (long long)r * runs;
+    float m = NEG;
+    for (int i = lane; i < runs; i += 64) m = fmaxf(m, p[i].x);
+    m = wave_max(m);
+    float s = 0.f;
+    for (int i = lane; i < runs; i += 64) s += rebased(p[i], m);
+    s = wave_sum(s);
+    if (lane != 0) return;
+    const long long tok = tokens[r];
+    lp[r] = tok >= 0 && tok < V ? log_prob_of(target[r], m, s) : 0.f;
+    stats[r] = make_float2(m, s);
+}
+
+// What the backward of a row is made of: dl_i = (others * exp(y_i - from) + [i = tok] at_token) * (factor of a seen token)
+struct Slope {
+    int tok;
+    bool zero;                       // a row without a token, or with none allowed
+    float at_token, others, from;
+    __device__ Slope(const Args &a, int r, const int64_t *tokens, const float2 *stats, const float *g, const Rule<float> &rule) {
+        const float2 st = stats[r];
+        tok = token_of(tokens[r], a.V), zero = tok < 0 || (st.x == NEG && st.y == 0.f);
+        at_token = g[r] * rule.scale, others = -at_token * reciprocal(st.y), from = reference_of(st.x);
+    }
+    template <int VEC> __device__ __forceinline__ void of(int i, float (&v)[VEC]) const {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[j] = others * exp_from(v[j], from);
+        const unsigned here = (unsigned)(tok - i);
+        if (here < (unsigned)VEC) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                if (j == (int)here) v[j] += at_token;
+        }
+    }
+};
+
+template <typename T, int K, bool BIAS>
+__global__ __launch_bounds__(NT) void log_prob_rows_bwd_kernel(Args a, const int64_t *__restrict__ tokens, const float2 *__restrict__ stats,
+                                                               const float *__restrict__ g, T *__restrict__ dx, long long ld_dx) {
+    using N = Narrow<T, K, BIAS>;
+    __shared__ __align__(16) typename N::Lds lds[WAVES];
+    N u(a, lds, (const T *)a.logits, a.ld_b, a.ld_t);
+    if (!u.live) return;
+    const Rule<float> rule(u.w, 1.f);
+    const Slope slope(a, u.r, tokens, stats, g, rule);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        float v[N::VEC];
+        u.values(k, rule, v);
+        slope.of(N::P::at(k), v);
+        int c[N::VEC];
+        if (u.counts(k, c)) {
+#pragma unroll
+            for (int j = 0; j < N::VEC; ++j)
+                if (c[j] > 0) v[j] *= rule.factor((float)u.p.x[k].v[j]);
+        }
+        if (slope.zero) u.p.allow[k] = 0u;
+        u.p.masked(k, 0.f, v);
+        store_pack(dx + u.r * ld_dx + N::P::at(k), rounded<T>(v), a.V - N::P::at(k));
+    }
+}
+
+// (The rows are taken from the last one down: what the forward pass read last is what the last-level cache still holds.)
+template <typename T, int K, bool BIAS>
+__global__ __launch_bounds__(NT) void log_prob_run_bwd_kernel(Args a, const int64_t *__restrict__ tokens, const float2 *__restrict__ stats,
+                                                              const float *__restrict__ g, T *__restrict__ dx, long long ld_dx) {
+    using P = Packs<T, K, BIAS>;
+    const Place at(a, gridDim.x - 1 - blockIdx.x);
+    const Row<T> w = row_of<T>(a, at.r);
+    const Rule<float> rule(w, 1.f);
+    Seen<float> seen(run_lds, a.run, a.L);
+    const Slope slope(a, at.r, tokens, stats, g, rule);
+    T *row = dx + at.r * ld_dx;
+    stream<P>(a, at, w, w.x, [&] { if (a.history) look_back<true>(seen, w, rule, at.base, at.n); },
+                 [&](const P &p, int first) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int i = first + P::at(k);
+            float v[P::VEC];
+            p.raw(k, rule, v);
+            slope.of(i, v);
+            const uint32_t allow = slope.zero ? 0u : p.allow[k];
+#pragma unroll
+            for (int j = 0; j < P::VEC; ++j) v[j] = select(bit_word(allow, j), v[j], 0.f);
+            store_pack(row + i, rounded<T>(v), a.V - i);
+        }
+    });
+    if (a.history) {
+        __syncthreads();             // (orders these stores after the stream's)
+        for (int u = threadIdx.x; u < seen.total; u += NT) {
+            const int i = at.base + seen.id[u];
+            float v[1] = {seen.value[u]};
+            slope.of(i, v);
+            row[i] = (T)(slope.zero || !w.allows(i) ? 0.f : v[0] * rule.factor((float)w.x[i]));
+        }
+    }
+}
+
+// ---- draw
+template <typename T, int K, bool BIAS>
+__global__ __launch_bounds__(NT) void draw_rows_kernel(Args a, const float *__restrict__ uniforms, long long ld_u, int64_t empty,
+                                                       int64_t *__restrict__ out, float *__restrict__ lp) {
+    using N = Narrow<T, K, BIAS>;
+    __shared__ __align__(16) typename N::Lds lds[WAVES];
+    N u(a, lds, (const T *)a.logits, a.ld_b, a.ld_t);
+    if (!u.live) return;
+    const Rule<double> rule(u.w, LOG2E64);
+    double e[K][N::VEC];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        u.values(k, rule, e[k]);
+        u.p.masked(k, NEG64, e[k]);
+    }
+    double top = NEG64;
+    bool bad = false;
+    largest(e, top, bad);
+    const double m = reference_of(top);
+    exponentials(e, m);
+    const double s = wave_sum(lane_sum(e));
+    const Pick pick = pick_in_wave(e, 0., (double)uniforms[u.r * ld_u] * s);
+    const bool nan = __ballot(bad) != 0;
+    if (u.lane == 0) {
+        const bool ok = s > 0. && m < __builtin_inf() && pick.index >= 0 && !nan;
+        out[u.r] = ok ? pick.index : empty;
+        lp[u.r] = ok ? draw_log_prob(pick.value, s) : (m == NEG64 && !nan ? NEG : __builtin_nanf(""));
+    }
+}
+
+// A wide row, first: every step of a run leaves the sum of its 2^(z - m) and its m.
+struct Piece {
+    double s, m;
+};
+template <typename T, int K, bool BIAS> __global__ __launch_bounds__(NT) void draw_run_kernel(Args a, Piece *__restrict__ part) {
+    using P = Packs<T, K, BIAS>;
+    const Place at(a, blockIdx.x);
+    const Row<T> w = row_of<T>(a, at.r);
+    const Rule<double> rule(w, LOG2E64);
+    Seen<double> seen(run_lds, a.run, a.L);
+    const int pieces = (a.V + P::SPAN - 1) / P::SPAN, lane = threadIdx.x & 63;
+    stream<P>(a, at, w, w.x, [&] { if (a.history) look_back<true>(seen, w, rule, at.base, at.n); },
+                 [&](const P &p, int first) {
+        double e[K][P::VEC], top = NEG64;
+        bool bad = false;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int i = first + P::at(k) - at.base;
+            p.raw(k, rule, e[k]);
+            uint32_t allow = p.allow[k];
+            if (a.history) allow &= ~seen_bits<P::VEC>(seen, i, at.n);
+#pragma unroll
+            for (int j = 0; j < P::VEC; ++j) e[k][j] = select(bit_word(allow, j), e[k][j], NEG64);
+        }
+        largest(e, top, bad);
+        int u0 = 0, u1 = 0;          // the list's entries of this step
+        if (a.history) {
+            const int word = (first - at.base) >> 5, next = word + P::SPAN / 32;
+            u0 = seen.rank[word], u1 = next < (at.n + 31) >> 5 ? seen.rank[next] : seen.total;
+            for (int u = u0 + lane; u < u1; u += 64) bad |= seen.value[u] != seen.value[u], top = fmax(top, seen.value[u]);
+        }
+        const double m = reference_of(top);
+        exponentials(e, m);
+        double s = lane_sum(e);
+        for (int u = u0 + lane; u < u1; u += 64) s += power_of_two(seen.value[u] - (m == NEG64 ? 0. : m));
+        s = wave_sum(s);
+        const bool nan = __ballot(bad) != 0;
+        if (lane == 0) part[(long long)at.r * pieces + first / P::SPAN] = Piece{s, nan ? __builtin_nan("") : m};
+    });
+}
+
+// Then one workgroup per row: the pieces joined in index order, the piece that holds u * total found, and its elements computed and walked
+// again, a few for each thread.
+template <typename T, int SPAN>
 __global__ __launch_bounds__(NT) void draw_join_kernel(Args a, const Piece *__restrict__ part, const float *__restrict__ uniforms,
-                                                       long long ld_u, int64_t empty, int64_t *__restrict__ out,
-                                                       float *__restrict__ lp) {
-    constexpr int VEC = Elem<T>::VEC, SPAN = 64 * VEC * K;             // a piece: what one wave of draw_piece_kernel had
-    constexpr int SLABS = K < WAVES ? 1 : K / WAVES, USED = K / SLABS;   // packs for each of the waves that take part
-    __shared__ __align__(16) std::conditional_t<HIST, Past<SPAN>, NoPast> past;
+                                                       long long ld_u, int64_t empty, int64_t *__restrict__ out, float *__restrict__ lp) {
+    constexpr int EACH = SPAN / NT;
+    __shared__ __align__(16) Counts<SPAN> lds;
     __shared__ double sums[WAVES];
     __shared__ Pick picks[WAVES];
-    const int r = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), pieces = a.units * WAVES;
+    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int pieces = (a.V + SPAN - 1) / SPAN;
     const Piece *p = part + (long long)r * pieces;
+    if (a.history) {
+        for (int i = tid; i < SPAN; i += NT) lds.cell[i] = 0;
+    }
     double m = NEG64;
     bool bad = false;
     for (int i = lane; i < pieces; i += 64) m = fmax(m, p[i].m), bad |= p[i].m != p[i].m;
     m = wave_max(m);
     const bool nan = __ballot(bad) != 0;
     if (nan || !(m > NEG64 && m < __builtin_inf())) {   // (the same in every wave)
-        if (threadIdx.x == 0) out[r] = empty, lp[r] = !nan && m == NEG64 ? NEG : __builtin_nanf("");
+        if (tid == 0) out[r] = empty, lp[r] = !nan && m == NEG64 ? NEG : __builtin_nanf("");
         return;
     }
     double total = 0.;
@@ -715,9 +987,9 @@ __global__ __launch_bounds__(NT) void draw_join_kernel(Args a, const Piece *__re
     double cum = 0., before = 0.;
     for (int base = 0; base < pieces && !over; base += 64) {
         const int i = base + lane;
-        const double w = i < pieces ? p[i].s * power_of_two(p[i].m - m) : 0.;
-        const double inc = wave_scan(w), ahead = cum + (inc - w);
-        const unsigned long long some = __ballot(w > 0.), hit = __ballot(w > 0. && cum + inc > thr);
+        const double s = i < pieces ? p[i].s * power_of_two(p[i].m - m) : 0.;
+        const double inc = wave_scan(s), ahead = cum + (inc - s);
+        const unsigned long long some = __ballot(s > 0.), hit = __ballot(s > 0. && cum + inc > thr);
         if (some) {
             const int l = hit ? __ffsll((long long)hit) - 1 : 63 - __clzll((long long)some);
             found = base + l, before = from_lane(ahead, l), over = hit != 0;
@@ -725,74 +997,85 @@ __global__ __launch_bounds__(NT) void draw_join_kernel(Args a, const Piece *__re
         cum += from_lane(inc, 63);
     }
     const Row<T> w = row_of<T>(a, r);
-    const int base = found * SPAN, n = a.V - base < SPAN ? a.V - base : SPAN;   // (a piece with a positive sum begins inside the row)
-    if constexpr (HIST) count_unit(past, w.hist, w.len, base, n, threadIdx.x, NT);
-    double e[SLABS][VEC];
-    double s = 0.;
-    if (wave < USED) {
-        const Rule<double> rule(w, LOG2E64);
+    const int base = found * SPAN, n = a.V - base < SPAN ? a.V - base : SPAN;
+    // this thread's elements, requested before the history is walked
+    const int mine = tid * EACH;
+    float x[EACH], b[EACH];
+    uint32_t allow = 0u;
 #pragma unroll
-        for (int k = 0; k < SLABS; ++k) {
-            const int at = ((wave * SLABS + k) * 64 + lane) * VEC, left = n - at, i = base + at;
-            const Pack<T> x = load_pack(w.x + i, left);
-            const uint32_t bits = left > 0 ? (w.mask ? w.mask[i >> 5] >> (i & 31) : 0xffffffffu) : 0u;
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                e[k][j] = 0.;
-                if (j < left && ((bits >> j) & 1u)) {
-                    double y = (double)(float)x.v[j];
-                    if constexpr (HIST) {
-                        if (past.cell[at + j] > 0) y = rule.penalised(y, past.cell[at + j]);
-                    }
-                    e[k][j] = power_of_two(scaled(y + (w.bias ? (double)w.bias[i + j] : 0.), rule.scale) - m);
-                }
-                s += e[k][j];
-            }
+    for (int j = 0; j < EACH; ++j) {
+        const bool in = mine + j < n;
+        x[j] = in ? (float)w.x[base + mine + j] : 0.f;
+        b[j] = in && w.bias ? w.bias[base + mine + j] : 0.f;
+        const bool yes = in && (!w.mask || ((w.mask[(base + mine + j) >> 5] >> ((base + mine + j) & 31)) & 1u));
+        allow |= (yes ? 1u : 0u) << j;
+    }
+    if (a.history) {
+        __syncthreads();
+#pragma unroll 4
+        for (int j = tid; j < w.len; j += NT) {
+            const unsigned long long at = (unsigned long long)(w.hist[j] - base);
+            if (at < (unsigned long long)n) atomicAdd(&lds.cell[at], 1);
         }
-        s = wave_sum(s);
-        if (lane == 0) sums[wave] = s;
+        __syncthreads();
     }
-    __syncthreads();
-    if (wave < USED) {
-        for (int v = 0; v < wave; ++v) before += sums[v];
-        const Pick pick = pick_in_wave(e, before, thr);
-        if (lane == 0) picks[wave] = pick;
+    const Rule<double> rule(w, LOG2E64);
+    double e[1][EACH];
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+        double y = (double)x[j];
+        if (a.history) {
+            const int c = lds.cell[mine + j];
+            if (c > 0) y = rule.penalised(y, c);
+        }
+        e[0][j] = (allow >> j) & 1u ? power_of_two(scaled(y + (double)b[j], rule.scale) - m) : 0.;
     }
+    const double s = wave_sum(lane_sum(e));
+    if (lane == 0) sums[wave] = s;
     __syncthreads();
-    if (threadIdx.x == 0) {
+    for (int v = 0; v < wave; ++v) before += sums[v];
+    const Pick pick = pick_in_wave(e, before, thr);
+    if (lane == 0) picks[wave] = pick;
+    __syncthreads();
+    if (tid == 0) {
         Pick best = {0., -1, false};
-        for (int v = 0; v < USED && !best.over; ++v)
-            if (picks[v].index >= 0) best = picks[v], best.index += v * SLABS * 64 * VEC;
+        for (int v = 0; v < WAVES && !best.over; ++v)
+            if (picks[v].index >= 0) best = picks[v], best.index += v * 64 * EACH;
         out[r] = best.index >= 0 ? base + best.index : empty;
         lp[r] = best.index >= 0 ? draw_log_prob(best.value, total) : __builtin_nanf("");
     }
 }
 
 // ---- host
-constexpr int ROW_MAX = 1024;        // widest vocabulary of the wave-per-row form
 constexpr long long MAX_BLOCKS = (1ll << 24) - 1;   // a launch holds fewer than 2^32 threads
 
 int elem_size(int dtype) { return dtype == PSVAE_F32 ? 4 : 2; }
 
-// How a call is cut: rows per workgroup and the loads per thread (as elements per thread, 8 .. 32).
+// How a call is cut.
 struct Cut {
-    bool wave_rows;
-    int per_thread, units;
+    bool rows;                       // a wave per row
+    int per_lane;                    // elements a lane takes at once: 8 or 16 (a row of up to 512 or 1024; a step)
+    int run, runs;                   // elements of a run, runs of a row
     long long blocks;
 };
 Cut cut_of(const psvae_shaping *s) {
     Cut c;
     const long long R = (long long)s->B * s->T;
-    c.wave_rows = s->V <= ROW_MAX;
-    if (c.wave_rows) {
-        c.per_thread = s->V <= 512 ? 8 : 16, c.units = 1;
+    c.rows = s->V <= ROW_MAX;
+    if (c.rows) {
+        c.per_lane = s->V <= 512 ? 8 : 16, c.run = s->V, c.runs = 1;
         c.blocks = (R + WAVES - 1) / WAVES;
         return c;
     }
-    // units of 8192 elements; of 2048 where those would leave compute units idle
-    c.per_thread = R * psvae_cdiv(s->V, NT * 32) < 512 ? 8 : 32;
-    c.units = psvae_cdiv(s->V, NT * c.per_thread);
-    c.blocks = R * c.units;
+    // The longest runs that leave 1024 workgroups, 4 for each compute unit (a run pays for its walk through the history once); down
+    // to 2048 elements, in smaller steps, where rows are few.  A long history's list of seen ids has to fit LDS: at most 4096 of them.
+    const int longest = s->history != nullptr && s->L > 4096 ? 4096 : RUN_MAX;
+    long long runs = std::max<long long>(psvae_cdiv(s->V, longest), std::min<long long>(psvae_cdiv(s->V, 2048), (1024 + R - 1) / std::max<long long>(R, 1)));
+    c.run = psvae_cdiv(psvae_cdiv(s->V, runs), 2048) * 2048;
+    if (c.run > 2048) c.run = psvae_cdiv(c.run, 4096) * 4096;
+    c.per_lane = c.run > 2048 ? 16 : 8;
+    c.runs = psvae_cdiv(s->V, c.run);
+    c.blocks = R * c.runs;
     return c;
 }
 
@@ -826,53 +1109,49 @@ int check_shaping(const char *fn, const psvae_shaping *s, Args *a) {
     a->rep = s->repetition, a->pres = s->presence, a->freq = s->frequency, a->temp = s->temperature;
     a->bias = s->bias, a->ld_bias = s->ld_bias;
     a->allowed = s->allowed, a->ld_allowed = s->ld_allowed, a->state = s->state, a->state_per_row = s->state_per_row;
-    a->units = cut_of(s).units;
+    const Cut c = cut_of(s);
+    a->run = c.run, a->runs = c.runs;
     return PSVAE_OK;
 }
 
-// Launches KERNEL<T, K, ROWS, HIST> for the call's type, cut and history.
-#define PSVAE_LAUNCH_K(KERNEL, T, K, ROWS, ...)                                                                                     \
+// Launches a kernel of the call's type, elements per lane and (where it has both forms) with or without a bias.  BYTES: dynamic LDS.
+#define PSVAE_LAUNCH_KERNEL(KERNEL, BYTES, ...) \
+    hipLaunchKernelGGL((KERNEL), dim3((unsigned)cut.blocks), dim3(NT), args.history ? (BYTES) : 0, st, __VA_ARGS__)
+#define PSVAE_LAUNCH(NAME, T, BYTES, ...)                                                                                           \
     do {                                                                                                                            \
-        if (args.history) hipLaunchKernelGGL((KERNEL<T, K, ROWS, true>), dim3((unsigned)cut.blocks), dim3(NT), 0, st, __VA_ARGS__); \
-        else hipLaunchKernelGGL((KERNEL<T, K, ROWS, false>), dim3((unsigned)cut.blocks), dim3(NT), 0, st, __VA_ARGS__);             \
+        if (cut.per_lane == 8 && args.bias) PSVAE_LAUNCH_KERNEL((NAME<T, 8 / Elem<T>::VEC, true>), BYTES, __VA_ARGS__);             \
+        else if (cut.per_lane == 8) PSVAE_LAUNCH_KERNEL((NAME<T, 8 / Elem<T>::VEC, false>), BYTES, __VA_ARGS__);                    \
+        else if (args.bias) PSVAE_LAUNCH_KERNEL((NAME<T, 16 / Elem<T>::VEC, true>), BYTES, __VA_ARGS__);                            \
+        else PSVAE_LAUNCH_KERNEL((NAME<T, 16 / Elem<T>::VEC, false>), BYTES, __VA_ARGS__);                                          \
     } while (0)
-#define PSVAE_LAUNCH_T(KERNEL, T, ...)                                                               \
-    do {                                                                                             \
-        constexpr int PER = Elem<T>::VEC;                                                            \
-        if (cut.wave_rows && cut.per_thread == 8) PSVAE_LAUNCH_K(KERNEL, T, 8 / PER, WAVES, __VA_ARGS__);   \
-        else if (cut.wave_rows) PSVAE_LAUNCH_K(KERNEL, T, 16 / PER, WAVES, __VA_ARGS__);             \
-        else if (cut.per_thread == 8) PSVAE_LAUNCH_K(KERNEL, T, 8 / PER, 1, __VA_ARGS__);            \
-        else PSVAE_LAUNCH_K(KERNEL, T, 32 / PER, 1, __VA_ARGS__);                                    \
+#define PSVAE_LAUNCH_NO_BIAS(NAME, T, BYTES, ...)                                                                  \
+    do {                                                                                                           \
+        if (cut.per_lane == 8) PSVAE_LAUNCH_KERNEL((NAME<T, 8 / Elem<T>::VEC>), BYTES, __VA_ARGS__);               \
+        else PSVAE_LAUNCH_KERNEL((NAME<T, 16 / Elem<T>::VEC>), BYTES, __VA_ARGS__);                                \
     } while (0)
-
-template <typename T, int K> void launch_draw_wide(const Args &args, const Cut &cut, Piece *part, const float *u, long long ld_u,
-                                                   int64_t empty, int64_t *out, float *lp, hipStream_t st) {
-    if (args.history) {
-        hipLaunchKernelGGL((draw_piece_kernel<T, K, true>), dim3((unsigned)cut.blocks), dim3(NT), 0, st, args, part);
-        hipLaunchKernelGGL((draw_join_kernel<T, K, true>), dim3((unsigned)args.R), dim3(NT), 0, st, args, part, u, ld_u, empty, out, lp);
-    } else {
-        hipLaunchKernelGGL((draw_piece_kernel<T, K, false>), dim3((unsigned)cut.blocks), dim3(NT), 0, st, args, part);
-        hipLaunchKernelGGL((draw_join_kernel<T, K, false>), dim3((unsigned)args.R), dim3(NT), 0, st, args, part, u, ld_u, empty, out, lp);
-    }
-}
 
 template <typename T> void launch_draw(const Args &args, const Cut &cut, Piece *part, const float *u, long long ld_u, int64_t empty,
                                        int64_t *out, float *lp, hipStream_t st) {
-    constexpr int PER = Elem<T>::VEC;
-    if (cut.wave_rows) {
-        if (cut.per_thread == 8) PSVAE_LAUNCH_K(draw_row_kernel, T, 8 / PER, WAVES, args, u, ld_u, empty, out, lp);
-        else PSVAE_LAUNCH_K(draw_row_kernel, T, 16 / PER, WAVES, args, u, ld_u, empty, out, lp);
-    } else if (cut.per_thread == 8) {
-        launch_draw_wide<T, 8 / PER>(args, cut, part, u, ld_u, empty, out, lp, st);
-    } else {
-        launch_draw_wide<T, 32 / PER>(args, cut, part, u, ld_u, empty, out, lp, st);
+    if (cut.rows) {
+        PSVAE_LAUNCH(draw_rows_kernel, T, 0, args, u, ld_u, empty, out, lp);
+        return;
     }
+    PSVAE_LAUNCH(draw_run_kernel, T, Seen<double>::bytes(args.run, args.L), args, part);
+    if (cut.per_lane == 8)
+        hipLaunchKernelGGL((draw_join_kernel<T, 512>), dim3((unsigned)args.R), dim3(NT), 0, st, args, part, u, ld_u, empty, out, lp);
+    else
+        hipLaunchKernelGGL((draw_join_kernel<T, 1024>), dim3((unsigned)args.R), dim3(NT), 0, st, args, part, u, ld_u, empty, out, lp);
 }
 
-size_t pieces_of(const psvae_shaping *s) {
-    if (s == nullptr || s->B <= 0 || s->T < 1 || s->V < 1) return 0;
+// parts of a wide call's rows: runs for a log-probability (none where one run is the row), steps for a draw
+bool sized(const psvae_shaping *s) { return s != nullptr && s->B > 0 && s->T >= 1 && s->V >= 1; }
+size_t log_prob_parts(const psvae_shaping *s) {
     const Cut c = cut_of(s);
-    return c.wave_rows ? 0 : (size_t)s->B * s->T * c.units * WAVES;
+    return c.runs > 1 ? (size_t)s->B * s->T * c.runs : 0;
+}
+size_t draw_parts(const psvae_shaping *s) {
+    const Cut c = cut_of(s);
+    return c.rows ? 0 : (size_t)s->B * s->T * psvae_cdiv(s->V, 64 * c.per_lane);
 }
 
 }  // namespace
@@ -893,7 +1172,12 @@ extern "C" int psvae_shape_logits_fwd(const psvae_shaping *shaping, void *out, i
     PSVAE_REQUIRE(((uintptr_t)out & (elem_size(shaping->dtype) - 1)) == 0, PSVAE_EINVAL, "%s: misaligned output", fn);
     const Cut cut = cut_of(shaping);
     hipStream_t st = (hipStream_t)stream;
-#define CALL(T) PSVAE_LAUNCH_T(shape_fwd_kernel, T, args, (T *)out, (long long)ld_out)
+    const size_t lds = Seen<float>::bytes(args.run, args.L);
+#define CALL(T)                                                                                       \
+    do {                                                                                              \
+        if (cut.rows) PSVAE_LAUNCH(shape_rows_kernel, T, 0, args, (T *)out, (long long)ld_out);     \
+        else PSVAE_LAUNCH(shape_run_kernel, T, lds, args, (T *)out, (long long)ld_out);           \
+    } while (0)
     PSVAE_BY_TYPE(CALL);
 #undef CALL
     PSVAE_CHECK_LAUNCH(fn);
@@ -910,7 +1194,13 @@ extern "C" int psvae_shape_logits_bwd(const psvae_shaping *shaping, const void *
     PSVAE_REQUIRE((((uintptr_t)g | (uintptr_t)dlogits) & (elem_size(shaping->dtype) - 1)) == 0, PSVAE_EINVAL, "%s: misaligned gradient", fn);
     const Cut cut = cut_of(shaping);
     hipStream_t st = (hipStream_t)stream;
-#define CALL(T) PSVAE_LAUNCH_T(shape_bwd_kernel, T, args, (const T *)g, (long long)ld_gb, (long long)ld_gt, (T *)dlogits, (long long)ld_dlogits)
+    const size_t lds = Seen<float>::bytes(args.run, 0);
+#define SHAPE_BWD(T) args, (const T *)g, (long long)ld_gb, (long long)ld_gt, (T *)dlogits, (long long)ld_dlogits
+#define CALL(T)                                                                     \
+    do {                                                                            \
+        if (cut.rows) PSVAE_LAUNCH_NO_BIAS(shape_rows_bwd_kernel, T, 0, SHAPE_BWD(T));    \
+        else PSVAE_LAUNCH_NO_BIAS(shape_run_bwd_kernel, T, lds, SHAPE_BWD(T));          \
+    } while (0)
     PSVAE_BY_TYPE(CALL);
 #undef CALL
     PSVAE_CHECK_LAUNCH(fn);
@@ -918,8 +1208,8 @@ extern "C" int psvae_shape_logits_bwd(const psvae_shaping *shaping, const void *
 }
 
 extern "C" size_t psvae_shaped_log_prob_workspace_bytes(const psvae_shaping *shaping) {
-    const size_t pieces = pieces_of(shaping);
-    return pieces ? pieces * sizeof(float2) + (size_t)shaping->B * shaping->T * sizeof(float) : 0;
+    const size_t parts = sized(shaping) ? log_prob_parts(shaping) : 0;
+    return parts ? parts * sizeof(float2) + (size_t)shaping->B * shaping->T * sizeof(float) : 0;
 }
 
 extern "C" int psvae_shaped_log_prob_fwd(const psvae_shaping *shaping, const int64_t *tokens, float *log_prob, float *stats,
@@ -936,13 +1226,18 @@ extern "C" int psvae_shaped_log_prob_fwd(const psvae_shaping *shaping, const int
     const Cut cut = cut_of(shaping);
     hipStream_t st = (hipStream_t)stream;
     float2 *part = (float2 *)workspace, *stat2 = (float2 *)stats;
-    float *target = need ? (float *)(part + pieces_of(shaping)) : nullptr;
-#define CALL(T) PSVAE_LAUNCH_T(log_prob_fwd_kernel, T, args, tokens, log_prob, stat2, part, target)
+    float *target = need ? (float *)(part + log_prob_parts(shaping)) : nullptr;
+    const size_t lds = Seen<float>::bytes(args.run, args.L);
+#define CALL(T)                                                                                               \
+    do {                                                                                                      \
+        if (cut.rows) PSVAE_LAUNCH(log_prob_rows_kernel, T, 0, args, tokens, log_prob, stat2);              \
+        else PSVAE_LAUNCH(log_prob_run_kernel, T, lds, args, tokens, log_prob, stat2, part, target);      \
+    } while (0)
     PSVAE_BY_TYPE(CALL);
 #undef CALL
     PSVAE_CHECK_LAUNCH(fn);
-    if (!cut.wave_rows) {
-        hipLaunchKernelGGL(log_prob_join_kernel, dim3(psvae_cdiv(args.R, WAVES)), dim3(NT), 0, st, args.R, args.V, args.units * WAVES,
+    if (need) {
+        hipLaunchKernelGGL(log_prob_join_kernel, dim3(psvae_cdiv(args.R, WAVES)), dim3(NT), 0, st, args.R, args.V, args.runs,
                            tokens, part, target, log_prob, stat2);
         PSVAE_CHECK_LAUNCH(fn);
     }
@@ -960,14 +1255,20 @@ extern "C" int psvae_shaped_log_prob_bwd(const psvae_shaping *shaping, const int
                   "%s: misaligned gradient or stats", fn);
     const Cut cut = cut_of(shaping);
     hipStream_t st = (hipStream_t)stream;
-#define CALL(T) PSVAE_LAUNCH_T(log_prob_bwd_kernel, T, args, tokens, (const float2 *)stats, g, (T *)dlogits, (long long)ld_dlogits)
+    const size_t lds = Seen<float>::bytes(args.run, args.L);
+#define LOG_PROB_BWD(T) args, tokens, (const float2 *)stats, g, (T *)dlogits, (long long)ld_dlogits
+#define CALL(T)                                                                           \
+    do {                                                                                  \
+        if (cut.rows) PSVAE_LAUNCH(log_prob_rows_bwd_kernel, T, 0, LOG_PROB_BWD(T));    \
+        else PSVAE_LAUNCH(log_prob_run_bwd_kernel, T, lds, LOG_PROB_BWD(T));          \
+    } while (0)
     PSVAE_BY_TYPE(CALL);
 #undef CALL
     PSVAE_CHECK_LAUNCH(fn);
     return PSVAE_OK;
 }
 
-extern "C" size_t psvae_shaped_draw_workspace_bytes(const psvae_shaping *shaping) { return pieces_of(shaping) * sizeof(Piece); }
+extern "C" size_t psvae_shaped_draw_workspace_bytes(const psvae_shaping *shaping) { return sized(shaping) ? draw_parts(shaping) * sizeof(Piece) : 0; }
 
 extern "C" int psvae_shaped_draw(const psvae_shaping *shaping, const float *uniforms, int64_t ld_uniforms, int64_t empty_token,
                                  int64_t *tokens, float *log_prob, void *workspace, size_t workspace_bytes, void *stream) {

@@ -89,7 +89,7 @@ def test_rejected_descriptions(L):
     assert fwd(desc(), out=None) == EINVAL and fwd(desc(), ld=301) == EINVAL and fwd(desc(), out=P + 2) == EINVAL
     assert fwd(desc(V=(1 << 30) + 1, ld_b=1 << 31), ld=1 << 31) == ETOOLARGE
     assert fwd(desc(B=1 << 20, T=1 << 12)) == ETOOLARGE               # 2^32 rows
-    assert fwd(desc(B=1 << 16, V=1 << 22, ld_b=1 << 22), ld=1 << 22) == ETOOLARGE   # more workgroups than a launch holds
+    assert fwd(desc(B=1 << 20, V=1 << 22, ld_b=1 << 22), ld=1 << 22) == ETOOLARGE   # more workgroups than a launch holds
 
     bwd = lambda s, g=P, d=P, ld=302: L.psvae_shape_logits_bwd(ctypes.byref(s), g, 302, 0, d, ld, None)   # noqa: E731
     assert bwd(desc(B=0)) == 0 and bwd(desc(), g=None) == EINVAL and bwd(desc(), d=None) == EINVAL and bwd(desc(), ld=300) == EINVAL
