@@ -122,6 +122,26 @@ template <typename T> __device__ __forceinline__ void store_pack(T *p, const Pac
     }
 }
 
+// f(id - base) for every id of a row's history that lies in [base, base + n): the threads `tid` of `threads` take it in turn, BATCH ids
+// of each requested at once (one by one, each behind the last one's test, a walk of 4000 ids took 16 memory latencies).  Ids outside
+// the vocabulary fall outside every range.
+template <int BATCH, typename F> __device__ __forceinline__ void walk(const int64_t *hist, int len, int base, int n, int tid, int threads, F f) {
+    for (int first = 0; first < len; first += BATCH * threads) {
+        int64_t id[BATCH];
+#pragma unroll
+        for (int q = 0; q < BATCH; ++q) {
+            const int j = first + q * threads + tid;
+            if (first + q * threads < len) id[q] = hist[j < len ? j : len - 1];
+        }
+#pragma unroll
+        for (int q = 0; q < BATCH; ++q) {
+            if (first + q * threads >= len) break;
+            const unsigned long long at = (unsigned long long)(id[q] - base);
+            if (first + q * threads + tid < len && at < (unsigned long long)n) f((int)at);
+        }
+    }
+}
+
 // ---- bits.  Bit j of `bits` as a word of ones or zeros: one bit-field extract, and a masked value is then one bit-select
 // (a compare and a conditional move per value would be three).
 __device__ __forceinline__ int bit_word(uint32_t bits, int j) { return (int)(bits << (31 - j)) >> 31; }
@@ -236,10 +256,11 @@ __device__ __forceinline__ float log_prob_of(float y_tok, float m, float s) {
 // exponentials and sums are 64-bit: the pick is the one of the exact distribution but for ~1e-8 of the rows, whatever the tiling.
 constexpr double NEG64 = -__builtin_inf(), LOG2E64 = 1.4426950408889634;
 
-// 2^z for z <= 0 (0 below 2^-1074): 2^n of the nearest whole number times a polynomial in the rest |r| <= 1/2 - the one of degree 9 that is 1
+// 2^z (0 below 2^-1074): 2^n of the nearest whole number times a polynomial in the rest |r| <= 1/2 - the one of degree 9 that is 1
 // at r = 0 and has the smallest largest relative error (Remez exchange: 7.7e-14).
 __device__ __forceinline__ double power_of_two(double z) {
-    z = fmax(z, -1080.);
+    double low = -1080.;
+    asm("v_max_f64 %0, %1, %2" : "=v"(z) : "v"(z), "s"(low));   // (fmax would first quieten z in an instruction of its own)
     const double n = rint(z), r = z - n;
     double p = 9.16811938851594e-08;
     p = fma(p, r, 1.3255182784592006e-06);
@@ -254,68 +275,117 @@ __device__ __forceinline__ double power_of_two(double z) {
     return ldexp(p, (int)n);
 }
 
-// The reference m of a wave's z (log2 e times y; -inf where not allowed) from each lane's largest: near or at the largest of all.
-__device__ __forceinline__ double reference_of(double top) {
-    // a 32-bit maximum serves while its rounding is small in z's units
-    const double m = (double)wave_max((float)top);
-    return fabs(m) < 1e6 ? m : wave_max(top);
+
+// -1080 in place of t where the bit is clear: its power of two is 0
+__device__ __forceinline__ double or_nothing(int word, double t) {
+    const unsigned long long x = (unsigned long long)__double_as_longlong(t);
+    const unsigned lo = (unsigned)x & (unsigned)word, hi = ((unsigned)(x >> 32) & (unsigned)word) | (0xc090e000u & ~(unsigned)word);
+    return __longlong_as_double((long long)(((unsigned long long)hi << 32) | lo));
 }
-template <int K, int VEC> __device__ __forceinline__ void largest(const double (&z)[K][VEC], double &top, bool &bad) {
+
+// The weights 2^(z - m) of a wave's elements, z = v * scale (scale: log2 e over the temperature), 0 where `allow` has no bit.  fill(k, v) gives
+// the v of pack k, take(k, weights) gets its weights, more(f) calls f for further z of this lane.
+// Any m will do that leaves the sum in range and comes to the same for equal rows, so m is the largest of 64 elements, each lane's first - its
+// product with the scale then needs no rounding of its own - and the largest of all (exactly: equal z have to give equal weights,
+// however large they are) only where these allow nothing, are not small numbers, or turn out to be far below the others.
+struct Weights {
+    double sum, m;                   // m: NaN if an allowed value is, +inf if one is, -inf if there is none
+};
+template <int K, int VEC, typename Fill, typename Take, typename More>
+__device__ __forceinline__ Weights weigh(const uint32_t (&allow)[K], double scale, Fill fill, Take take, More more) {
+    double v[VEC];
+    fill(0, v);
+    double m = (double)wave_max(allow[0] & 1u ? (float)(v[0] * scale) : NEG), sum = __builtin_nan("");
+    bool bad = false;
+    if (fabs(m) < 1e6) {
+        sum = 0.;
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+        for (int k = 0; k < K; ++k) {
+            if (k > 0) fill(k, v);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) bad |= z[k][j] != z[k][j], top = fmax(top, z[k][j]);
-}
-// z becomes 2^(z - m), 0 where not allowed
-template <int K, int VEC> __device__ __forceinline__ void exponentials(double (&z)[K][VEC], double m) {
-    const double from = m == NEG64 ? 0. : m;
+            for (int j = 0; j < VEC; ++j) {
+                v[j] = or_nothing(bit_word(allow[k], j), fma(v[j], scale, -m));
+                bad |= v[j] != v[j];
+                v[j] = power_of_two(v[j]);
+                sum += v[j];
+            }
+            take(k, v);
+        }
+        more([&](double z) { bad |= z != z, sum += power_of_two(z - m); });
+        sum = wave_sum(sum);
+    }
+    if (!(sum < 0x1p500)) {
+        double largest = NEG64;
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+        for (int k = 0; k < K; ++k) {
+            fill(k, v);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) z[k][j] = power_of_two(z[k][j] - from);
-}
-template <int K, int VEC> __device__ __forceinline__ double lane_sum(const double (&e)[K][VEC]) {
-    double s = 0.;
+            for (int j = 0; j < VEC; ++j) {
+                v[j] = select(bit_word(allow[k], j), scaled(v[j], scale), NEG64);
+                bad |= v[j] != v[j], largest = fmax(largest, v[j]);
+            }
+        }
+        more([&](double z) { bad |= z != z, largest = fmax(largest, z); });
+        m = wave_max(largest);
+        const double from = m == NEG64 ? 0. : m;
+        sum = 0.;
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+        for (int k = 0; k < K; ++k) {
+            fill(k, v);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) s += e[k][j];
-    return s;
+            for (int j = 0; j < VEC; ++j) v[j] = power_of_two(select(bit_word(allow[k], j), scaled(v[j], scale), NEG64) - from), sum += v[j];
+            take(k, v);
+        }
+        more([&](double z) { sum += power_of_two(z - from); });
+        sum = wave_sum(sum);
+    }
+    return {sum, __ballot(bad) ? __builtin_nan("") : m};
 }
 
 // The first element, in index order, at which the running sum (starting from `before`) exceeds thr; the last positive one if it never
-// does.  Returns whether it did, the element's index inside the wave's piece (-1: nothing positive) and its e.  The whole wave calls it.
+// does: lane l holds the weights of elements l * N .. l * N + N - 1.  Returns whether it did, the element's index (-1: nothing
+// positive) and its weight.  The whole wave calls it.
 struct Pick {
     double value;
     int index;
     bool over;
 };
-template <int K, int VEC> __device__ __forceinline__ Pick pick_in_wave(const double (&e)[K][VEC], double before, double thr) {
-    Pick found = {0., -1, false};
-    double cum = before;
+template <int N> __device__ __forceinline__ Pick pick_in_wave(const double (&e)[N], double before, double thr) {
+    double s = 0.;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        double s = 0.;
+    for (int j = 0; j < N; ++j) s += e[j];
+    const double inc = wave_scan(s);
+    const unsigned long long some = __ballot(s > 0.), hit = __ballot(s > 0. && before + inc > thr);
+    if (!some) return {0., -1, false};
+    // inside each lane: the first positive element past thr, else the last positive one
+    int mine = -1;
+    double run = before + (inc - s), v = 0.;
+    bool over = false;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) s += e[k][j];
-        const double inc = wave_scan(s);
-        const unsigned long long some = __ballot(s > 0.), hit = __ballot(s > 0. && cum + inc > thr);
-        if (!found.over && some) {
-            // inside each lane: the first positive element past thr, else the last positive one
-            int mine = -1;
-            double run = cum + (inc - s), v = 0.;
-            bool over = false;
-#pragma unroll
-            for (int j = 0; j < VEC; ++j)
-                if (e[k][j] > 0. && !over) run += e[k][j], mine = j, v = e[k][j], over = run > thr;
-            const int l = hit ? __ffsll((long long)hit) - 1 : 63 - __clzll((long long)some);
-            found.index = (k * 64 + l) * VEC + __builtin_amdgcn_readlane(mine, l), found.value = from_lane(v, l), found.over = hit != 0;
-        }
-        cum += from_lane(inc, 63);
-    }
-    return found;
+    for (int j = 0; j < N; ++j)
+        if (e[j] > 0. && !over) run += e[j], mine = j, v = e[j], over = run > thr;
+    const int l = hit ? __ffsll((long long)hit) - 1 : 63 - __clzll((long long)some);
+    return {from_lane(v, l), l * N + __builtin_amdgcn_readlane(mine, l), hit != 0};
 }
-__device__ __forceinline__ float draw_log_prob(double value, double total) { return (float)log(value / total); }
+
+// log q for q in (0, 1]: q = 2^n f with f in [sqrt(1/2), sqrt(2)), log f = 2 artanh(s), s = (f - 1) / (f + 1), |s| < 0.172: the series to s^15 leaves
+// less than 1e-14 of the value.
+__device__ __forceinline__ double log_of(double q) {
+    int n;
+    double f = frexp(q, &n);
+    if (f < 0.70710678118654752) f *= 2., --n;
+    const double s = (f - 1.) * reciprocal(f + 1.), t = s * s;
+    double p = 1. / 15.;
+    p = fma(p, t, 1. / 13.);
+    p = fma(p, t, 1. / 11.);
+    p = fma(p, t, 1. / 9.);
+    p = fma(p, t, 1. / 7.);
+    p = fma(p, t, 1. / 5.);
+    p = fma(p, t, 1. / 3.);
+    p = fma(p, t, 1.);
+    return fma((double)n, 0.69314718055994531, 2. * s * p);
+}
+__device__ __forceinline__ float draw_log_prob(double value, double total) { return (float)log_of(value == total ? 1. : value * reciprocal(total)); }
 
 // ---- packs: K of them are a thread's share of 64 * VEC * K neighbouring elements, pack k holding elements (k * 64 + lane) * VEC of these.
 template <typename T, int K, bool BIAS> struct Packs {
@@ -358,15 +428,23 @@ template <typename T, int K, bool BIAS> struct Packs {
         }
     }
     // y as if nothing had been seen, before the mask
-    template <typename C> __device__ __forceinline__ void raw(int k, const Rule<C> &rule, C (&y)[VEC]) const {
+    __device__ __forceinline__ void raw(int k, const Rule<float> &rule, float (&y)[VEC]) const {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-            y[j] = (C)(float)x[k].v[j];
-            if constexpr (BIAS) y[j] += (C)b[k][j];
+            y[j] = (float)x[k].v[j];
+            if constexpr (BIAS) y[j] += b[k][j];
             y[j] = scaled(y[j], rule.scale);
         }
     }
-    template <typename C> __device__ __forceinline__ void masked(int k, C no, C (&y)[VEC]) const {
+    // the same before the last factor, in 64 bits
+    __device__ __forceinline__ void sums(int k, double (&v)[VEC]) const {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            v[j] = (double)(float)x[k].v[j];
+            if constexpr (BIAS) v[j] += (double)b[k][j];
+        }
+    }
+    __device__ __forceinline__ void masked(int k, float no, float (&y)[VEC]) const {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) y[j] = select(bit_word(allow[k], j), y[j], no);
     }
@@ -378,64 +456,98 @@ template <typename T, int VEC> __device__ __forceinline__ Pack<T> rounded(const 
     return p;
 }
 
-// ---- rows of at most ROW_MAX elements: a wave each.  The counts of all ids are a dense array.
+// ---- rows of at most ROW_MAX elements: a wave each, a lane holding N neighbouring elements, N = V / 64 rounded up to a form that is
+// built.  (One form of 8, its loads aligned, leaves 2 lanes in 5 idle at 300 elements.)  The counts of all ids are a dense array.
 constexpr int ROW_MAX = 1024;
 template <int SPAN> struct Counts {
     int cell[SPAN];
 };
+template <typename T, int N> struct __attribute__((packed, aligned(sizeof(T)))) Few { T v[N]; };
 
-template <typename T, int K, bool BIAS> struct Narrow {
-    using P = Packs<T, K, BIAS>;
-    using Lds = Counts<P::SPAN>;
-    static constexpr int VEC = P::VEC;
-    int r, lane;
-    bool live, past;
+template <typename T, int N> struct Narrow {
+    using Lds = Counts<64 * N>;
+    int r, lane, i, left;            // i: the lane's first element; left: elements of the row from it on
+    bool live;
     Row<T> w;
-    P p;
-    Lds *lds;
+    Few<T, N> x;                     // logits (or what `from` holds)
+    Few<float, N> b;                 // bias, 0 without one
+    uint32_t allow;                  // bit j: element i + j is in the row and allowed
+    const int *cell;                 // counts of the lane's elements; null: no history
     __device__ Narrow(const Args &a, Lds *all, const T *from, long long ld_b, long long ld_t) {
         const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-        lane = threadIdx.x & 63, r = blockIdx.x * WAVES + wave, live = r < a.R, past = a.history != nullptr, lds = all + wave;
+        lane = threadIdx.x & 63, r = blockIdx.x * WAVES + wave, live = r < a.R, i = lane * N, left = a.V - i;
         if (!live) r = a.R - 1;      // (such a wave only keeps the barriers company)
         w = row_of<T>(a, r);
-        const int b = a.T == 1 ? r : (int)((unsigned)r / (unsigned)a.T), t = r - b * a.T;
-        p.load_end(from + b * ld_b + t * ld_t, w, 0, a.V);
-        if (past) {
-            for (int i = lane * 4; i < P::SPAN; i += 256) *reinterpret_cast<int4 *>(lds->cell + i) = make_int4(0, 0, 0, 0);
-            __syncthreads();
-#pragma unroll 4
-            for (int j = lane; j < w.len; j += 64) {
-                const unsigned long long id = (unsigned long long)w.hist[j];
-                if (id < (unsigned long long)a.V) atomicAdd(&lds->cell[id], 1);
-            }
-            __syncthreads();
-        }
-    }
-    // the counts of pack k; whether any lane of the wave has one above 0
-    __device__ __forceinline__ bool counts(int k, int (&c)[VEC]) const {
-        if (!past) return false;
-        int any = 0;
-#pragma unroll
-        for (int q = 0; q < VEC / 4; ++q) {
-            const int4 v = *reinterpret_cast<const int4 *>(lds->cell + P::at(k) + 4 * q);
-            c[4 * q] = v.x, c[4 * q + 1] = v.y, c[4 * q + 2] = v.z, c[4 * q + 3] = v.w;
-            any |= (v.x | v.y) | (v.z | v.w);
-        }
-        return __ballot(any != 0) != 0;
-    }
-    // y of pack k, before the mask
-    template <typename C> __device__ __forceinline__ void values(int k, const Rule<C> &rule, C (&y)[VEC]) const {
-        int c[VEC];
-        if (counts(k, c)) {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const C x = (C)(float)p.x[k].v[j];
-                y[j] = c[j] > 0 ? rule.penalised(x, c[j]) : x;
-                if constexpr (BIAS) y[j] += (C)p.b[k][j];
-                y[j] = scaled(y[j], rule.scale);
-            }
+        const int seq = a.T == 1 ? r : (int)((unsigned)r / (unsigned)a.T), t = r - seq * a.T;
+        from += seq * ld_b + t * ld_t;
+        allow = w.none || left <= 0 ? 0u : left >= N ? 0xffffffffu : (1u << left) - 1u;
+        if (left >= N) {
+            x = *reinterpret_cast<const Few<T, N> *>(from + i);
         } else {
-            p.raw(k, rule, y);
+#pragma unroll
+            for (int j = 0; j < N; ++j) x.v[j] = j < left ? from[i + j] : (T)0.f;
+        }
+        if (!w.bias) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) b.v[j] = 0.f;
+        } else if (left >= N) {
+            b = *reinterpret_cast<const Few<float, N> *>(w.bias + i);
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j) b.v[j] = j < left ? w.bias[i + j] : 0.f;
+        }
+        if (w.mask && left > 0) {    // (the bits may lie in two words)
+            const int last = (a.V - 1) >> 5, word = i >> 5;
+            const unsigned long long two = w.mask[word] | (unsigned long long)w.mask[word < last ? word + 1 : last] << 32;
+            allow &= (uint32_t)(two >> (i & 31));
+        }
+        cell = nullptr;
+        if (a.history) {
+            int *cells = all[wave].cell;
+            for (int q = lane; q < 64 * N; q += 64) cells[q] = 0;
+            __syncthreads();
+            walk<4>(w.hist, w.len, 0, a.V, lane, 64, [&](int id) { atomicAdd(&cells[id], 1); });
+            __syncthreads();
+            cell = cells + i;
+        }
+    }
+    // logits with the penalties and the bias: y before the last factor
+    template <typename C> __device__ __forceinline__ void sums(const Rule<C> &rule, C (&v)[N]) const {
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = (C)(float)x.v[j];
+        if (cell) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const int c = cell[j];
+                v[j] = c > 0 ? rule.penalised(v[j], c) : v[j];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] += (C)b.v[j];
+    }
+    __device__ __forceinline__ void values(const Rule<float> &rule, float no, float (&y)[N]) const {
+        sums(rule, y);
+#pragma unroll
+        for (int j = 0; j < N; ++j) y[j] = select(bit_word(allow, j), scaled(y[j], rule.scale), no);
+    }
+    // d y / d l of a seen element's logit l: what its gradient is multiplied by
+    __device__ __forceinline__ void times_factor(const Rule<float> &rule, const Few<T, N> &l, float (&v)[N]) const {
+        if (cell) {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (cell[j] > 0) v[j] *= rule.factor((float)l.v[j]);
+        }
+    }
+    __device__ __forceinline__ void store(T *row, const float (&v)[N]) const {
+        if (left >= N) {
+            Few<T, N> p;
+#pragma unroll
+            for (int j = 0; j < N; ++j) p.v[j] = (T)v[j];
+            *reinterpret_cast<Few<T, N> *>(row + i) = p;
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (j < left) row[i + j] = (T)v[j];
         }
     }
 };
@@ -446,52 +558,38 @@ template <typename T, int K, bool BIAS> struct Narrow {
 template <typename C> struct Seen {
     C *value;
     uint32_t *bits;
-    uint16_t *rank, *id;
-    int total;                       // entries of the list
+    uint16_t *rank, *small;
+    int total, cap;                  // entries of the list; room in it
+    // Beside entry u's count (which `value` holds first) there are two 16-bit numbers: its id, and - while the list is made - one of the
+    // history's ids in the run, in any order.  A double has room for them in itself (the id is not asked for after the value is there).
+    static constexpr int BESIDE = sizeof(C) == 8 ? 0 : 4;
     static size_t bytes(int run, int len) {
         const int cap = len < run ? len : run;
-        return ((size_t)cap * (sizeof(C) + 2) + 15) / 16 * 16 + (size_t)run / 32 * 6;
+        return ((size_t)cap * (sizeof(C) + BESIDE) + 15) / 16 * 16 + (size_t)run / 32 * 6;
     }
-    __device__ Seen(char *lds, int run, int len) : total(0) {
-        const int cap = len < run ? len : run;
-        value = reinterpret_cast<C *>(lds), id = reinterpret_cast<uint16_t *>(lds + (size_t)cap * sizeof(C));
-        bits = reinterpret_cast<uint32_t *>(lds + ((size_t)cap * (sizeof(C) + 2) + 15) / 16 * 16);
+    __device__ Seen(char *lds, int run, int len) : total(0), cap(len < run ? len : run) {
+        value = reinterpret_cast<C *>(lds), small = reinterpret_cast<uint16_t *>(lds + (BESIDE ? (size_t)cap * sizeof(C) : 0));
+        bits = reinterpret_cast<uint32_t *>(lds + ((size_t)cap * (sizeof(C) + BESIDE) + 15) / 16 * 16);
         rank = reinterpret_cast<uint16_t *>(bits + run / 32);
     }
+    __device__ __forceinline__ uint16_t &id(int u) const { return small[BESIDE ? u : 4 * u + 2]; }
+    __device__ __forceinline__ uint16_t &hit(int u) const { return small[BESIDE ? cap + u : 4 * u + 3]; }
 };
 
 constexpr int RUN_MAX = 32768;       // ranks and ids fit 16 bits; 1024 words of bits, 4 for each thread
-constexpr int HELD = 4;              // ids of the history that a thread keeps between the walks
-
-// One walk over the row's history: f(element of the run) for every id in it.
-template <typename F> __device__ __forceinline__ void walk(const int (&held)[HELD], const int64_t *hist, int len, int base, int n, F f) {
-#pragma unroll
-    for (int q = 0; q < HELD; ++q)
-        if (held[q] >= 0) f(held[q]);
-#pragma unroll 4
-    for (int j = HELD * NT + threadIdx.x; j < len; j += NT) {
-        const unsigned long long at = (unsigned long long)(hist[j] - base);   // ids outside the vocabulary fall outside every run
-        if (at < (unsigned long long)n) f((int)at);
-    }
-}
-
 // Sets the bits of the seen elements of [base, base + n); with LIST also ranks and the list of finished values.  The workgroup calls it.
 template <bool LIST, typename T, typename C>
 __device__ __forceinline__ void look_back(Seen<C> &seen, const Row<T> &w, const Rule<C> &rule, int base, int n) {
-    __shared__ int wave_total[WAVES];
+    __shared__ int wave_total[WAVES], hits;
     const int words = (n + 31) >> 5, tid = threadIdx.x;
-    int held[HELD];
-#pragma unroll
-    for (int q = 0; q < HELD; ++q) {
-        held[q] = -1;
-        if (tid + q * NT < w.len) {
-            const unsigned long long at = (unsigned long long)(w.hist[tid + q * NT] - base);
-            if (at < (unsigned long long)n) held[q] = (int)at;
-        }
-    }
+    const bool kept = LIST && w.len <= seen.cap;   // the ids found are kept, for the second time
     for (int i = tid; i < words; i += NT) seen.bits[i] = 0u;
+    if (tid == 0) hits = 0;
     __syncthreads();
-    walk(held, w.hist, w.len, base, n, [&](int at) { atomicOr(&seen.bits[at >> 5], 1u << (at & 31)); });
+    walk<8>(w.hist, w.len, base, n, tid, NT, [&](int at) {
+        atomicOr(&seen.bits[at >> 5], 1u << (at & 31));
+        if (kept) seen.hit(atomicAdd(&hits, 1)) = (uint16_t)at;
+    });
     __syncthreads();
     if constexpr (LIST) {
         // ranks: every thread 4 words, their bits counted and summed over the workgroup
@@ -517,19 +615,24 @@ __device__ __forceinline__ void look_back(Seen<C> &seen, const Row<T> &w, const 
             const int i = tid * (RUN_MAX / 32 / NT) + q;
             if (i < words) seen.rank[i] = (uint16_t)(first + here[q]);
         }
-        int *count = reinterpret_cast<int *>(seen.value);   // cell u of the list: first its count, in the cell's first 4 bytes
+        int *count = reinterpret_cast<int *>(seen.value);   // entry u: first its count, in the value's first 4 bytes
         constexpr int STEP = sizeof(C) / 4;
         for (int u = tid; u < total; u += NT) count[u * STEP] = 0;
         __syncthreads();
-        walk(held, w.hist, w.len, base, n, [&](int at) {
+        auto count_one = [&](int at) {
             const uint32_t word = seen.bits[at >> 5];
             const int u = seen.rank[at >> 5] + __popc(word & ((1u << (at & 31)) - 1u));
             atomicAdd(&count[u * STEP], 1);
-            seen.id[u] = (uint16_t)at;                       // (the same from every thread that holds the id)
-        });
+            seen.id(u) = (uint16_t)at;                       // (the same from every thread that holds the id)
+        };
+        if (kept) {
+            for (int j = tid; j < hits; j += NT) count_one(seen.hit(j));
+        } else {
+            walk<8>(w.hist, w.len, base, n, tid, NT, count_one);
+        }
         __syncthreads();
         for (int u = tid; u < total; u += NT) {
-            const int at = seen.id[u], i = base + at;
+            const int at = seen.id(u), i = base + at;
             const C v = rule.penalised((C)(float)w.x[i], count[u * STEP]) + (w.bias ? (C)w.bias[i] : (C)0);
             seen.value[u] = w.allows(i) ? scaled(v, rule.scale) : (C)NEG;
         }
@@ -582,20 +685,13 @@ __device__ __forceinline__ void stream(const Args &a, const Place &at, const Row
 extern __shared__ __align__(16) char run_lds[];
 
 // ---- shape
-template <typename T, int K, bool BIAS>
-__global__ __launch_bounds__(NT) void shape_rows_kernel(Args a, T *__restrict__ out, long long ld_out) {
-    using N = Narrow<T, K, BIAS>;
-    __shared__ __align__(16) typename N::Lds lds[WAVES];
-    N u(a, lds, (const T *)a.logits, a.ld_b, a.ld_t);
+template <typename T, int N> __global__ __launch_bounds__(NT) void shape_rows_kernel(Args a, T *__restrict__ out, long long ld_out) {
+    __shared__ typename Narrow<T, N>::Lds lds[WAVES];
+    const Narrow<T, N> u(a, lds, (const T *)a.logits, a.ld_b, a.ld_t);
     if (!u.live) return;
-    const Rule<float> rule(u.w, 1.f);
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-        float v[N::VEC];
-        u.values(k, rule, v);
-        u.p.masked(k, NEG, v);
-        store_pack(out + u.r * ld_out + N::P::at(k), rounded<T>(v), a.V - N::P::at(k));
-    }
+    float v[N];
+    u.values(Rule<float>(u.w, 1.f), NEG, v);
+    u.store(out + u.r * ld_out, v);
 }
 
 template <typename T, int K, bool BIAS> __global__ __launch_bounds__(NT) void shape_run_kernel(Args a, T *__restrict__ out, long long ld_out) {
@@ -618,32 +714,30 @@ template <typename T, int K, bool BIAS> __global__ __launch_bounds__(NT) void sh
     });
     if (a.history) {
         __syncthreads();             // (orders these stores after the stream's)
-        for (int u = threadIdx.x; u < seen.total; u += NT) row[at.base + seen.id[u]] = (T)seen.value[u];
+        for (int u = threadIdx.x; u < seen.total; u += NT) row[at.base + seen.id(u)] = (T)seen.value[u];
     }
 }
 
 // dl = g dy/dl; the logits are read only where the sign of a seen token's decides.
-template <typename T, int K>
+template <typename T, int N>
 __global__ __launch_bounds__(NT) void shape_rows_bwd_kernel(Args a, const T *__restrict__ g, long long ld_gb, long long ld_gt,
                                                             T *__restrict__ dx, long long ld_dx) {
-    using N = Narrow<T, K, false>;
-    __shared__ __align__(16) typename N::Lds lds[WAVES];
-    N u(a, lds, g, ld_gb, ld_gt);
+    __shared__ typename Narrow<T, N>::Lds lds[WAVES];
+    a.bias = nullptr;
+    const Narrow<T, N> u(a, lds, g, ld_gb, ld_gt);
     if (!u.live) return;
     const Rule<float> rule(u.w, 1.f);
+    float v[N];
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        float v[N::VEC];
-        u.p.raw(k, rule, v);
-        int c[N::VEC];
-        if (u.counts(k, c)) {
+    for (int j = 0; j < N; ++j) v[j] = (float)u.x.v[j] * rule.scale;
+    if (u.cell) {
 #pragma unroll
-            for (int j = 0; j < N::VEC; ++j)
-                if (c[j] > 0) v[j] *= rule.factor((float)u.w.x[N::P::at(k) + j]);
-        }
-        u.p.masked(k, 0.f, v);
-        store_pack(dx + u.r * ld_dx + N::P::at(k), rounded<T>(v), a.V - N::P::at(k));
+        for (int j = 0; j < N; ++j)
+            if (u.cell[j] > 0) v[j] *= rule.factor((float)u.w.x[u.i + j]);
     }
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = select(bit_word(u.allow, j), v[j], 0.f);
+    u.store(dx + u.r * ld_dx, v);
 }
 
 template <typename T, int K>
@@ -678,37 +772,27 @@ __global__ __launch_bounds__(NT) void shape_run_bwd_kernel(Args a, const T *__re
 
 // ---- log_prob.  Sums are 32-bit: a lane's at most 128 terms of a run in a chain (rescaled where its maximum grows), 6 levels over
 // the wave, 4 waves, then the row's runs: the relative error stays below (128 + 10 + runs) * 2^-24 and is far below it on average.
-template <typename T, int K, bool BIAS>
+template <typename T, int N>
 __global__ __launch_bounds__(NT) void log_prob_rows_kernel(Args a, const int64_t *__restrict__ tokens, float *__restrict__ lp,
                                                            float2 *__restrict__ stats) {
-    using N = Narrow<T, K, BIAS>;
-    __shared__ __align__(16) typename N::Lds lds[WAVES];
-    N u(a, lds, (const T *)a.logits, a.ld_b, a.ld_t);
+    __shared__ typename Narrow<T, N>::Lds lds[WAVES];
+    const Narrow<T, N> u(a, lds, (const T *)a.logits, a.ld_b, a.ld_t);
     if (!u.live) return;
-    const Rule<float> rule(u.w, 1.f);
     const int tok = token_of(tokens[u.r], a.V);
-    float y[K][N::VEC], m = NEG, yt = 0.f;
-    bool mine = false;
+    float y[N], m = NEG, yt = 0.f;
+    u.values(Rule<float>(u.w, 1.f), NEG, y);
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        u.values(k, rule, y[k]);
-        u.p.masked(k, NEG, y[k]);
-#pragma unroll
-        for (int j = 0; j < N::VEC; ++j) {
-            m = fmaxf(m, y[k][j]);
-            if (tok == N::P::at(k) + j) yt = y[k][j], mine = true;
-        }
+    for (int j = 0; j < N; ++j) {
+        m = fmaxf(m, y[j]);
+        if (u.i + j == tok) yt = y[j];
     }
     m = wave_max(m);
     const float from = reference_of(m);
     float s = 0.f;
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int j = 0; j < N::VEC; ++j) s += exp_from(y[k][j], from);
+    for (int j = 0; j < N; ++j) s += exp_from(y[j], from);
     s = wave_sum(s);
-    const unsigned long long owner = __ballot(mine);
-    const float v = owner ? log_prob_of(from_lane(yt, __ffsll((long long)owner) - 1), m, s) : 0.f;
+    const float v = tok >= 0 ? log_prob_of(from_lane(yt, tok / N), m, s) : 0.f;
     if (u.lane == 0) lp[u.r] = v, stats[u.r] = make_float2(m, s);
 }
 
@@ -758,7 +842,7 @@ __global__ __launch_bounds__(NT) void log_prob_run_kernel(Args a, const int64_t 
         for (int u = threadIdx.x; u < seen.total; u += NT) {
             const float y = seen.value[u], top = fmaxf(m, y), from = reference_of(top);
             s = s * exp_from(m, from) + exp_from(y, from), m = top;
-            if (at.base + seen.id[u] == tok) at_token = y;
+            if (at.base + seen.id(u) == tok) at_token = y;
         }
     }
     const float top = wave_max(m);
@@ -818,30 +902,22 @@ struct Slope {
     }
 };
 
-template <typename T, int K, bool BIAS>
+template <typename T, int N>
 __global__ __launch_bounds__(NT) void log_prob_rows_bwd_kernel(Args a, const int64_t *__restrict__ tokens, const float2 *__restrict__ stats,
                                                                const float *__restrict__ g, T *__restrict__ dx, long long ld_dx) {
-    using N = Narrow<T, K, BIAS>;
-    __shared__ __align__(16) typename N::Lds lds[WAVES];
-    N u(a, lds, (const T *)a.logits, a.ld_b, a.ld_t);
+    __shared__ typename Narrow<T, N>::Lds lds[WAVES];
+    const Narrow<T, N> u(a, lds, (const T *)a.logits, a.ld_b, a.ld_t);
     if (!u.live) return;
     const Rule<float> rule(u.w, 1.f);
     const Slope slope(a, u.r, tokens, stats, g, rule);
+    float v[N];
+    u.values(rule, NEG, v);
+    slope.of(u.i, v);
+    u.times_factor(rule, u.x, v);
+    const uint32_t allow = slope.zero ? 0u : u.allow;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        float v[N::VEC];
-        u.values(k, rule, v);
-        slope.of(N::P::at(k), v);
-        int c[N::VEC];
-        if (u.counts(k, c)) {
-#pragma unroll
-            for (int j = 0; j < N::VEC; ++j)
-                if (c[j] > 0) v[j] *= rule.factor((float)u.p.x[k].v[j]);
-        }
-        if (slope.zero) u.p.allow[k] = 0u;
-        u.p.masked(k, 0.f, v);
-        store_pack(dx + u.r * ld_dx + N::P::at(k), rounded<T>(v), a.V - N::P::at(k));
-    }
+    for (int j = 0; j < N; ++j) v[j] = select(bit_word(allow, j), v[j], 0.f);
+    u.store(dx + u.r * ld_dx, v);
 }
 
 // (The rows are taken from the last one down: what the forward pass read last is what the last-level cache still holds.)
@@ -872,7 +948,7 @@ __global__ __launch_bounds__(NT) void log_prob_run_bwd_kernel(Args a, const int6
     if (a.history) {
         __syncthreads();             // (orders these stores after the stream's)
         for (int u = threadIdx.x; u < seen.total; u += NT) {
-            const int i = at.base + seen.id[u];
+            const int i = at.base + seen.id(u);
             float v[1] = {seen.value[u]};
             slope.of(i, v);
             row[i] = (T)(slope.zero || !w.allows(i) ? 0.f : v[0] * rule.factor((float)w.x[i]));
@@ -881,36 +957,32 @@ __global__ __launch_bounds__(NT) void log_prob_run_bwd_kernel(Args a, const int6
 }
 
 // ---- draw
-template <typename T, int K, bool BIAS>
+template <typename T, int N>
 __global__ __launch_bounds__(NT) void draw_rows_kernel(Args a, const float *__restrict__ uniforms, long long ld_u, int64_t empty,
                                                        int64_t *__restrict__ out, float *__restrict__ lp) {
-    using N = Narrow<T, K, BIAS>;
-    __shared__ __align__(16) typename N::Lds lds[WAVES];
-    N u(a, lds, (const T *)a.logits, a.ld_b, a.ld_t);
+    __shared__ typename Narrow<T, N>::Lds lds[WAVES];
+    const Narrow<T, N> u(a, lds, (const T *)a.logits, a.ld_b, a.ld_t);
     if (!u.live) return;
     const Rule<double> rule(u.w, LOG2E64);
-    double e[K][N::VEC];
+    double v[N], e[N];
+    u.sums(rule, v);
+    const uint32_t allow[1] = {u.allow};
+    const Weights all = weigh<1, N>(allow, rule.scale, [&](int, double (&to)[N]) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        u.values(k, rule, e[k]);
-        u.p.masked(k, NEG64, e[k]);
-    }
-    double top = NEG64;
-    bool bad = false;
-    largest(e, top, bad);
-    const double m = reference_of(top);
-    exponentials(e, m);
-    const double s = wave_sum(lane_sum(e));
-    const Pick pick = pick_in_wave(e, 0., (double)uniforms[u.r * ld_u] * s);
-    const bool nan = __ballot(bad) != 0;
+        for (int j = 0; j < N; ++j) to[j] = v[j];
+    }, [&](int, const double (&from)[N]) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) e[j] = from[j];
+    }, [](auto) {});
+    const Pick pick = pick_in_wave(e, 0., (double)uniforms[u.r * ld_u] * all.sum);
     if (u.lane == 0) {
-        const bool ok = s > 0. && m < __builtin_inf() && pick.index >= 0 && !nan;
+        const bool ok = all.sum > 0. && fabs(all.m) < __builtin_inf() && pick.index >= 0;
         out[u.r] = ok ? pick.index : empty;
-        lp[u.r] = ok ? draw_log_prob(pick.value, s) : (m == NEG64 && !nan ? NEG : __builtin_nanf(""));
+        lp[u.r] = ok ? draw_log_prob(pick.value, all.sum) : (all.m == NEG64 ? NEG : __builtin_nanf(""));
     }
 }
 
-// A wide row, first: every step of a run leaves the sum of its 2^(z - m) and its m.
+// A wide row, first: every step of a run leaves the sum of its weights and its m.
 struct Piece {
     double s, m;
 };
@@ -923,31 +995,22 @@ template <typename T, int K, bool BIAS> __global__ __launch_bounds__(NT) void dr
     const int pieces = (a.V + P::SPAN - 1) / P::SPAN, lane = threadIdx.x & 63;
     stream<P>(a, at, w, w.x, [&] { if (a.history) look_back<true>(seen, w, rule, at.base, at.n); },
                  [&](const P &p, int first) {
-        double e[K][P::VEC], top = NEG64;
-        bool bad = false;
+        uint32_t allow[K];
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const int i = first + P::at(k) - at.base;
-            p.raw(k, rule, e[k]);
-            uint32_t allow = p.allow[k];
-            if (a.history) allow &= ~seen_bits<P::VEC>(seen, i, at.n);
-#pragma unroll
-            for (int j = 0; j < P::VEC; ++j) e[k][j] = select(bit_word(allow, j), e[k][j], NEG64);
+            allow[k] = p.allow[k];
+            if (a.history) allow[k] &= ~seen_bits<P::VEC>(seen, first + P::at(k) - at.base, at.n);
         }
-        largest(e, top, bad);
         int u0 = 0, u1 = 0;          // the list's entries of this step
         if (a.history) {
             const int word = (first - at.base) >> 5, next = word + P::SPAN / 32;
             u0 = seen.rank[word], u1 = next < (at.n + 31) >> 5 ? seen.rank[next] : seen.total;
-            for (int u = u0 + lane; u < u1; u += 64) bad |= seen.value[u] != seen.value[u], top = fmax(top, seen.value[u]);
         }
-        const double m = reference_of(top);
-        exponentials(e, m);
-        double s = lane_sum(e);
-        for (int u = u0 + lane; u < u1; u += 64) s += power_of_two(seen.value[u] - (m == NEG64 ? 0. : m));
-        s = wave_sum(s);
-        const bool nan = __ballot(bad) != 0;
-        if (lane == 0) part[(long long)at.r * pieces + first / P::SPAN] = Piece{s, nan ? __builtin_nan("") : m};
+        const Weights all = weigh<K, P::VEC>(allow, rule.scale, [&](int k, double (&v)[P::VEC]) { p.sums(k, v); }, [](int, auto &) {},
+                                             [&](auto f) {
+            for (int u = u0 + lane; u < u1; u += 64) f(seen.value[u]);
+        });
+        if (lane == 0) part[(long long)at.r * pieces + first / P::SPAN] = Piece{all.sum, all.m};
     });
 }
 
@@ -1012,15 +1075,11 @@ __global__ __launch_bounds__(NT) void draw_join_kernel(Args a, const Piece *__re
     }
     if (a.history) {
         __syncthreads();
-#pragma unroll 4
-        for (int j = tid; j < w.len; j += NT) {
-            const unsigned long long at = (unsigned long long)(w.hist[j] - base);
-            if (at < (unsigned long long)n) atomicAdd(&lds.cell[at], 1);
-        }
+        walk<8>(w.hist, w.len, base, n, tid, NT, [&](int at) { atomicAdd(&lds.cell[at], 1); });
         __syncthreads();
     }
     const Rule<double> rule(w, LOG2E64);
-    double e[1][EACH];
+    double e[EACH], s = 0.;
 #pragma unroll
     for (int j = 0; j < EACH; ++j) {
         double y = (double)x[j];
@@ -1028,9 +1087,9 @@ __global__ __launch_bounds__(NT) void draw_join_kernel(Args a, const Piece *__re
             const int c = lds.cell[mine + j];
             if (c > 0) y = rule.penalised(y, c);
         }
-        e[0][j] = (allow >> j) & 1u ? power_of_two(scaled(y + (double)b[j], rule.scale) - m) : 0.;
+        e[j] = (allow >> j) & 1u ? power_of_two(scaled(y + (double)b[j], rule.scale) - m) : 0., s += e[j];
     }
-    const double s = wave_sum(lane_sum(e));
+    s = wave_sum(s);
     if (lane == 0) sums[wave] = s;
     __syncthreads();
     for (int v = 0; v < wave; ++v) before += sums[v];
@@ -1054,7 +1113,7 @@ int elem_size(int dtype) { return dtype == PSVAE_F32 ? 4 : 2; }
 // How a call is cut.
 struct Cut {
     bool rows;                       // a wave per row
-    int per_lane;                    // elements a lane takes at once: 8 or 16 (a row of up to 512 or 1024; a step)
+    int per_lane;                    // elements a lane takes at once: of a row 1 to 16, of a run's step 8 or 16
     int run, runs;                   // elements of a run, runs of a row
     long long blocks;
 };
@@ -1063,7 +1122,11 @@ Cut cut_of(const psvae_shaping *s) {
     const long long R = (long long)s->B * s->T;
     c.rows = s->V <= ROW_MAX;
     if (c.rows) {
-        c.per_lane = s->V <= 512 ? 8 : 16, c.run = s->V, c.runs = 1;
+        c.run = s->V, c.runs = 1;
+        for (int n : {1, 2, 3, 4, 5, 6, 8, 12, 16}) {   // (the forms of PSVAE_LAUNCH_ROWS)
+            c.per_lane = n;
+            if (64 * n >= s->V) break;
+        }
         c.blocks = (R + WAVES - 1) / WAVES;
         return c;
     }
@@ -1071,8 +1134,8 @@ Cut cut_of(const psvae_shaping *s) {
     // to 2048 elements, in smaller steps, where rows are few.  A long history's list of seen ids has to fit LDS: at most 4096 of them.
     const int longest = s->history != nullptr && s->L > 4096 ? 4096 : RUN_MAX;
     long long runs = std::max<long long>(psvae_cdiv(s->V, longest), std::min<long long>(psvae_cdiv(s->V, 2048), (1024 + R - 1) / std::max<long long>(R, 1)));
-    c.run = psvae_cdiv(psvae_cdiv(s->V, runs), 2048) * 2048;
-    if (c.run > 2048) c.run = psvae_cdiv(c.run, 4096) * 4096;
+    c.run = psvae_cdiv(psvae_cdiv(s->V, runs), 1024) * 1024;
+    if (c.run < 2048) c.run = 2048;
     c.per_lane = c.run > 2048 ? 16 : 8;
     c.runs = psvae_cdiv(s->V, c.run);
     c.blocks = R * c.runs;
@@ -1124,6 +1187,20 @@ int check_shaping(const char *fn, const psvae_shaping *s, Args *a) {
         else if (args.bias) PSVAE_LAUNCH_KERNEL((NAME<T, 16 / Elem<T>::VEC, true>), BYTES, __VA_ARGS__);                            \
         else PSVAE_LAUNCH_KERNEL((NAME<T, 16 / Elem<T>::VEC, false>), BYTES, __VA_ARGS__);                                          \
     } while (0)
+#define PSVAE_LAUNCH_ROWS(NAME, T, ...)                                                      \
+    do {                                                                                     \
+        switch (cut.per_lane) {                                                              \
+            case 1: PSVAE_LAUNCH_KERNEL((NAME<T, 1>), 0, __VA_ARGS__); break;                \
+            case 2: PSVAE_LAUNCH_KERNEL((NAME<T, 2>), 0, __VA_ARGS__); break;                \
+            case 3: PSVAE_LAUNCH_KERNEL((NAME<T, 3>), 0, __VA_ARGS__); break;                \
+            case 4: PSVAE_LAUNCH_KERNEL((NAME<T, 4>), 0, __VA_ARGS__); break;                \
+            case 5: PSVAE_LAUNCH_KERNEL((NAME<T, 5>), 0, __VA_ARGS__); break;                \
+            case 6: PSVAE_LAUNCH_KERNEL((NAME<T, 6>), 0, __VA_ARGS__); break;                \
+            case 8: PSVAE_LAUNCH_KERNEL((NAME<T, 8>), 0, __VA_ARGS__); break;                \
+            case 12: PSVAE_LAUNCH_KERNEL((NAME<T, 12>), 0, __VA_ARGS__); break;              \
+            default: PSVAE_LAUNCH_KERNEL((NAME<T, 16>), 0, __VA_ARGS__); break;              \
+        }                                                                                    \
+    } while (0)
 #define PSVAE_LAUNCH_NO_BIAS(NAME, T, BYTES, ...)                                                                  \
     do {                                                                                                           \
         if (cut.per_lane == 8) PSVAE_LAUNCH_KERNEL((NAME<T, 8 / Elem<T>::VEC>), BYTES, __VA_ARGS__);               \
@@ -1133,7 +1210,7 @@ int check_shaping(const char *fn, const psvae_shaping *s, Args *a) {
 template <typename T> void launch_draw(const Args &args, const Cut &cut, Piece *part, const float *u, long long ld_u, int64_t empty,
                                        int64_t *out, float *lp, hipStream_t st) {
     if (cut.rows) {
-        PSVAE_LAUNCH(draw_rows_kernel, T, 0, args, u, ld_u, empty, out, lp);
+        PSVAE_LAUNCH_ROWS(draw_rows_kernel, T, args, u, ld_u, empty, out, lp);
         return;
     }
     PSVAE_LAUNCH(draw_run_kernel, T, Seen<double>::bytes(args.run, args.L), args, part);
@@ -1175,7 +1252,7 @@ extern "C" int psvae_shape_logits_fwd(const psvae_shaping *shaping, void *out, i
     const size_t lds = Seen<float>::bytes(args.run, args.L);
 #define CALL(T)                                                                                       \
     do {                                                                                              \
-        if (cut.rows) PSVAE_LAUNCH(shape_rows_kernel, T, 0, args, (T *)out, (long long)ld_out);     \
+        if (cut.rows) PSVAE_LAUNCH_ROWS(shape_rows_kernel, T, args, (T *)out, (long long)ld_out);     \
         else PSVAE_LAUNCH(shape_run_kernel, T, lds, args, (T *)out, (long long)ld_out);           \
     } while (0)
     PSVAE_BY_TYPE(CALL);
@@ -1198,7 +1275,7 @@ extern "C" int psvae_shape_logits_bwd(const psvae_shaping *shaping, const void *
 #define SHAPE_BWD(T) args, (const T *)g, (long long)ld_gb, (long long)ld_gt, (T *)dlogits, (long long)ld_dlogits
 #define CALL(T)                                                                     \
     do {                                                                            \
-        if (cut.rows) PSVAE_LAUNCH_NO_BIAS(shape_rows_bwd_kernel, T, 0, SHAPE_BWD(T));    \
+        if (cut.rows) PSVAE_LAUNCH_ROWS(shape_rows_bwd_kernel, T, SHAPE_BWD(T));    \
         else PSVAE_LAUNCH_NO_BIAS(shape_run_bwd_kernel, T, lds, SHAPE_BWD(T));          \
     } while (0)
     PSVAE_BY_TYPE(CALL);
@@ -1230,7 +1307,7 @@ extern "C" int psvae_shaped_log_prob_fwd(const psvae_shaping *shaping, const int
     const size_t lds = Seen<float>::bytes(args.run, args.L);
 #define CALL(T)                                                                                               \
     do {                                                                                                      \
-        if (cut.rows) PSVAE_LAUNCH(log_prob_rows_kernel, T, 0, args, tokens, log_prob, stat2);              \
+        if (cut.rows) PSVAE_LAUNCH_ROWS(log_prob_rows_kernel, T, args, tokens, log_prob, stat2);              \
         else PSVAE_LAUNCH(log_prob_run_kernel, T, lds, args, tokens, log_prob, stat2, part, target);      \
     } while (0)
     PSVAE_BY_TYPE(CALL);
@@ -1259,7 +1336,7 @@ extern "C" int psvae_shaped_log_prob_bwd(const psvae_shaping *shaping, const int
 #define LOG_PROB_BWD(T) args, tokens, (const float2 *)stats, g, (T *)dlogits, (long long)ld_dlogits
 #define CALL(T)                                                                           \
     do {                                                                                  \
-        if (cut.rows) PSVAE_LAUNCH(log_prob_rows_bwd_kernel, T, 0, LOG_PROB_BWD(T));    \
+        if (cut.rows) PSVAE_LAUNCH_ROWS(log_prob_rows_bwd_kernel, T, LOG_PROB_BWD(T));    \
         else PSVAE_LAUNCH(log_prob_run_bwd_kernel, T, lds, LOG_PROB_BWD(T));          \
     } while (0)
     PSVAE_BY_TYPE(CALL);
