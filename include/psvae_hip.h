@@ -587,12 +587,12 @@ int psvae_shaped_draw(const psvae_shaping *shaping, const float *uniforms, int64
  * src/train.py:47), for gradients that do not sit in one flat float32 buffer.  Lists are HOST arrays of n
  * entries, read before the call returns: device pointers, element counts (0 allowed) and types
  * (PSVAE_F32 / BF16 / F16).
- *   norm = sqrt(sum of squares), squares and sums in 64 bits, in an order that only the counts decide;
+ *   norm = sqrt(sum of squares), squares and sums in 64 bits, in an order that only counts and types decide;
  *   out_i = grad_i * min(1, max_norm / (norm + 1e-6))  (a NaN norm makes every value NaN)
  * out_i may be grad_i itself (then a factor of 1 writes nothing) and may be of another type; otherwise no
  * output may overlap a gradient or another output.
  * ---------------------------------------------------------------------------------- */
-size_t psvae_grad_norm_workspace_bytes(int n, const int64_t *numel_host);
+size_t psvae_grad_norm_workspace_bytes(int n);
 int psvae_grad_norm(int n, const void *const *grads_host, const int64_t *numel_host, const int32_t *types_host,
                     float *norm, void *workspace, size_t workspace_bytes, void *stream);
 int psvae_clip_grads(int n, const void *const *grads_host, const int64_t *numel_host, const int32_t *types_host,

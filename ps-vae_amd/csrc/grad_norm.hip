@@ -3,10 +3,11 @@
 //     norm = sqrt(sum_i sum_j g_ij^2);   out_ij = g_ij * min(1, max_norm / (norm + 1e-6))
 //
 // Bound by HBM at large sizes (one read for the norm, one read and one write for the scaling), by launches at small ones.  The list
-// travels as kernel arguments (up to LIST tensors a launch), so nothing is copied to the device, nothing outlives the call and a captured
-// graph holds its own copy.  Every tensor is cut into chunks of one size; a workgroup takes one chunk.  Squares are
-// formed and added in 64 bits: a float's square neither overflows nor vanishes there, and the card does a 64-bit multiply-add
-// at the rate of a 32-bit one, so the sum stays under the time of the loads.
+// travels as kernel arguments (up to 200 tensors a launch for the norm, 140 for the scaling), so nothing is copied to the device, nothing
+// outlives the call and a captured graph holds its own copy.  Every tensor is cut into chunks of so many BYTES - half as many elements
+// of a type twice as wide, so that the workgroups finish together - and up to 1024 workgroups a launch take the chunks in turn,
+// each with one partial sum at its end.  Squares are formed and added in 64 bits: a float's square neither overflows nor vanishes
+// there, and the card does a 64-bit multiply-add at the rate of a 32-bit one, so the sum stays under the time of the loads.
 #include "common.h"
 
 #include <algorithm>
@@ -16,19 +17,25 @@
 namespace {
 
 constexpr int NT = 256;
-constexpr int LIST = 120;                       // tensors per launch: 30 bytes each of the 4 KB that kernel arguments may take
-constexpr long long CHUNK_MIN = 4096;           // elements per workgroup: 16 per thread
-constexpr int PARTIALS = 2048;                  // workgroups that a large list is cut into (8 per compute unit)
+constexpr int GROUPS = 1024;                    // workgroups of a launch at most: 4 for each compute unit
+// Bytes of a chunk: 4 loads of a thread; 16 where a list is large, whose workgroups take many chunks (finding a chunk's tensor costs about a
+// microsecond's latency).
+constexpr int CHUNK_SMALL = NT * 16 * 4, CHUNK_LARGE = NT * 16 * 16;
+constexpr long long LARGE = 64ll << 20;         // bytes of a large list
 
-struct List {
-    const void *src[LIST];
-    void *dst[LIST];
-    long long numel[LIST];
-    int first[LIST + 1];                        // first chunk of each tensor, counted from the launch's first; [n]: chunks in all
-    uint8_t st[LIST], dt[LIST];
-    int n;
-    long long chunk;
+// A list's part for one launch.  `size`: the elements, with the source's type in bits 60, 61 and the output's in bits 62, 63.  `first`: the
+// tensor's first chunk, counted from the launch's first; [n]: chunks in all.
+template <int N, bool OUT> struct List {
+    static constexpr int ROOM = N;
+    const void *src[N];
+    void *dst[OUT ? N : 1];
+    unsigned long long size[N];
+    int first[N + 1];
+    int n, chunk;                               // tensors; bytes of a chunk
 };
+using NormList = List<200, false>;              // 20 bytes each of the 4 KB that kernel arguments may take
+using ClipList = List<140, true>;               // 28 bytes
+constexpr unsigned long long ELEMENTS = (1ull << 60) - 1;
 
 template <typename T> struct Elem;
 template <> struct Elem<float> { static constexpr int VEC = 4; };
@@ -49,25 +56,28 @@ __device__ __forceinline__ double block_sum(double s, double *sh) {
     return t;
 }
 
-// the tensor that chunk `c` of the launch belongs to
-__device__ __forceinline__ int tensor_of(const List &l, int c) {
+// Chunk c of the launch: f(tensor, source type, output type, first element, elements).
+template <typename L, typename F> __device__ __forceinline__ void with_chunk(const L &l, int c, F f) {
     int lo = 0, hi = l.n;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (l.first[mid] <= c) lo = mid;
         else hi = mid;
     }
-    return lo;
+    const unsigned long long size = l.size[lo];
+    const int st = (int)(size >> 60) & 3, each = st == PSVAE_F32 ? l.chunk / 4 : l.chunk / 2;
+    const long long at = (long long)(c - l.first[lo]) * each, left = (long long)(size & ELEMENTS) - at;
+    f(lo, st, (int)(size >> 62), at, left < each ? (int)left : each);
 }
 
-template <typename T> __device__ __forceinline__ double sum_squares(const T *g, long long n) {
+template <typename T> __device__ __forceinline__ double sum_squares(const T *g, int n) {
     constexpr int VEC = Elem<T>::VEC, UNROLL = 4;
     double acc[UNROLL] = {0., 0., 0., 0.};
-    long long i = (long long)threadIdx.x * VEC;
-    for (; i + (long long)(UNROLL - 1) * NT * VEC + VEC <= n; i += (long long)UNROLL * NT * VEC) {
+    int i = threadIdx.x * VEC;
+    for (; i + (UNROLL - 1) * NT * VEC + VEC <= n; i += UNROLL * NT * VEC) {
         Pack<T, VEC> p[UNROLL];
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) p[u] = *reinterpret_cast<const Pack<T, VEC> *>(g + i + (long long)u * NT * VEC);
+        for (int u = 0; u < UNROLL; ++u) p[u] = *reinterpret_cast<const Pack<T, VEC> *>(g + i + u * NT * VEC);
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u)
 #pragma unroll
@@ -76,8 +86,8 @@ template <typename T> __device__ __forceinline__ double sum_squares(const T *g, 
                 acc[u] = fma(d, d, acc[u]);
             }
     }
-    for (; i < n; i += (long long)NT * VEC) {
-        const int left = n - i < VEC ? (int)(n - i) : VEC;
+    for (; i < n; i += NT * VEC) {
+        const int left = n - i < VEC ? n - i : VEC;
         if (left == VEC) {
             const Pack<T, VEC> p = *reinterpret_cast<const Pack<T, VEC> *>(g + i);
 #pragma unroll
@@ -89,16 +99,17 @@ template <typename T> __device__ __forceinline__ double sum_squares(const T *g, 
     return (acc[0] + acc[1]) + (acc[2] + acc[3]);
 }
 
-__global__ __launch_bounds__(NT) void grad_squares_kernel(List l, double *__restrict__ partial) {
+__global__ __launch_bounds__(NT) void grad_squares_kernel(NormList l, double *__restrict__ partial) {
     __shared__ double sh[NT / 64];
-    const int c = blockIdx.x, i = tensor_of(l, c);
-    const long long at = (long long)(c - l.first[i]) * l.chunk, n = l.numel[i] - at < l.chunk ? l.numel[i] - at : l.chunk;
-    double s;
-    if (l.st[i] == PSVAE_F32) s = sum_squares((const float *)l.src[i] + at, n);
-    else if (l.st[i] == PSVAE_BF16) s = sum_squares((const __bf16 *)l.src[i] + at, n);
-    else s = sum_squares((const _Float16 *)l.src[i] + at, n);
+    double s = 0.;
+    for (int c = blockIdx.x; c < l.first[l.n]; c += gridDim.x)
+        with_chunk(l, c, [&](int i, int st, int, long long at, int n) {
+            if (st == PSVAE_F32) s += sum_squares((const float *)l.src[i] + at, n);
+            else if (st == PSVAE_BF16) s += sum_squares((const __bf16 *)l.src[i] + at, n);
+            else s += sum_squares((const _Float16 *)l.src[i] + at, n);
+        });
     s = block_sum(s, sh);
-    if (threadIdx.x == 0) partial[c] = s;
+    if (threadIdx.x == 0) partial[blockIdx.x] = s;
 }
 
 // The sum of all partials in one fixed order, the same in every workgroup that forms it.
@@ -115,73 +126,69 @@ __global__ __launch_bounds__(NT) void grad_norm_kernel(const double *__restrict_
     if (threadIdx.x == 0) *norm = (float)sqrt(s);
 }
 
-template <typename S, typename D> __device__ __forceinline__ void scale(const S *g, D *out, long long n, float coef) {
-    constexpr int VEC = Elem<S>::VEC, UNROLL = 4;
-    long long i = (long long)threadIdx.x * VEC;
-    for (; i + (long long)(UNROLL - 1) * NT * VEC + VEC <= n; i += (long long)UNROLL * NT * VEC) {
+// Loads and stores of at most 16 bytes a lane, so that a wave's store covers whole lines.
+// (Non-temporal: the scaled values are read by a later kernel, far more of them than the caches hold.)
+typedef uint32_t Words4 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t Words2 __attribute__((ext_vector_type(2), aligned(2)));
+template <typename T, int N> __device__ __forceinline__ void store_streamed(T *p, const Pack<T, N> &v) {
+    if constexpr (sizeof(v) == 8) __builtin_nontemporal_store(__builtin_bit_cast(Words2, v), reinterpret_cast<Words2 *>(p));
+    else __builtin_nontemporal_store(__builtin_bit_cast(Words4, v), reinterpret_cast<Words4 *>(p));
+}
+
+template <typename S, typename D> __device__ __forceinline__ void scale(const S *g, D *out, int n, float coef) {
+    constexpr int VEC = 16 / (sizeof(S) > sizeof(D) ? sizeof(S) : sizeof(D)), UNROLL = 64 / (VEC * (int)sizeof(S));
+    int i = threadIdx.x * VEC;
+    for (; i + (UNROLL - 1) * NT * VEC + VEC <= n; i += UNROLL * NT * VEC) {
         Pack<S, VEC> p[UNROLL];
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) p[u] = *reinterpret_cast<const Pack<S, VEC> *>(g + i + (long long)u * NT * VEC);
+        for (int u = 0; u < UNROLL; ++u) p[u] = *reinterpret_cast<const Pack<S, VEC> *>(g + i + u * NT * VEC);
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
             Pack<D, VEC> o;
 #pragma unroll
             for (int j = 0; j < VEC; ++j) o.v[j] = (D)((float)p[u].v[j] * coef);
-            *reinterpret_cast<Pack<D, VEC> *>(out + i + (long long)u * NT * VEC) = o;
+            store_streamed(out + i + u * NT * VEC, o);
         }
     }
-    for (; i < n; i += (long long)NT * VEC) {
-        const int left = n - i < VEC ? (int)(n - i) : VEC;
+    for (; i < n; i += NT * VEC) {
+        const int left = n - i < VEC ? n - i : VEC;
         for (int j = 0; j < left; ++j) out[i + j] = (D)((float)g[i + j] * coef);
     }
 }
 
-template <typename S> __device__ __forceinline__ void scale_to(const S *g, void *out, int dt, long long at, long long n, float coef) {
+template <typename S> __device__ __forceinline__ void scale_to(const S *g, void *out, int dt, long long at, int n, float coef) {
     if (dt == PSVAE_F32) scale(g + at, (float *)out + at, n, coef);
     else if (dt == PSVAE_BF16) scale(g + at, (__bf16 *)out + at, n, coef);
     else scale(g + at, (_Float16 *)out + at, n, coef);
 }
 
 // The chunks are taken from the list's end: what the norm read last is what the last-level cache still holds.
-__global__ __launch_bounds__(NT) void clip_grads_kernel(List l, const double *__restrict__ partial, int n_partial, float max_norm,
+__global__ __launch_bounds__(NT) void clip_grads_kernel(ClipList l, const double *__restrict__ partial, int n_partial, float max_norm,
                                                         float *__restrict__ norm) {
     __shared__ double sh[NT / 64];
     const double v = sqrt(total_of(partial, n_partial, sh));
-    if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)v;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)v;
     const double q = (double)max_norm / (v + 1e-6);
     const float coef = q > 1. ? 1.f : (float)q;   // (a NaN stays one, as torch.clamp keeps it)
-    const int c = (int)gridDim.x - 1 - (int)blockIdx.x;
-    const int i = tensor_of(l, c);
-    if (coef == 1.f && l.src[i] == l.dst[i] && l.st[i] == l.dt[i]) return;
-    const long long at = (long long)(c - l.first[i]) * l.chunk, n = l.numel[i] - at < l.chunk ? l.numel[i] - at : l.chunk;
-    if (l.st[i] == PSVAE_F32) scale_to((const float *)l.src[i], l.dst[i], l.dt[i], at, n, coef);
-    else if (l.st[i] == PSVAE_BF16) scale_to((const __bf16 *)l.src[i], l.dst[i], l.dt[i], at, n, coef);
-    else scale_to((const _Float16 *)l.src[i], l.dst[i], l.dt[i], at, n, coef);
+    for (int c = l.first[l.n] - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x)
+        with_chunk(l, c, [&](int i, int st, int dt, long long at, int n) {
+            if (coef == 1.f && l.src[i] == l.dst[i] && st == dt) return;
+            if (st == PSVAE_F32) scale_to((const float *)l.src[i], l.dst[i], dt, at, n, coef);
+            else if (st == PSVAE_BF16) scale_to((const __bf16 *)l.src[i], l.dst[i], dt, at, n, coef);
+            else scale_to((const _Float16 *)l.src[i], l.dst[i], dt, at, n, coef);
+        });
 }
 
 // ---- host
-// How a list is cut: the chunk length (a multiple of 64 elements) and the chunks.
-struct Cut {
-    long long chunk, chunks;
-};
-Cut cut_of(int n, const int64_t *numel) {
-    long long total = 0;
-    for (int i = 0; i < n; ++i) total += numel[i];
-    Cut c;
-    c.chunk = std::max(CHUNK_MIN, ((total + PARTIALS - 1) / PARTIALS + 63) / 64 * 64);
-    c.chunks = 0;
-    for (int i = 0; i < n; ++i) c.chunks += (numel[i] + c.chunk - 1) / c.chunk;
-    return c;
-}
-
 int type_size(int t) { return t == PSVAE_F32 ? 4 : 2; }
 
 int check_list(const char *fn, int n, const void *const *grads, const int64_t *numel, const int32_t *types) {
     PSVAE_REQUIRE(n >= 0, PSVAE_EINVAL, "%s: %d tensors", fn, n);
     PSVAE_REQUIRE(n == 0 || (grads && numel && types), PSVAE_EINVAL, "%s: null list", fn);
     PSVAE_REQUIRE(n <= (1 << 20), PSVAE_ETOOLARGE, "%s: %d tensors (at most 2^20)", fn, n);
+    long long total = 0;             // (at most 2^40 elements: 2^26 chunks)
     for (int i = 0; i < n; ++i) {
-        PSVAE_REQUIRE(numel[i] >= 0 && numel[i] < (1ll << 40), PSVAE_EINVAL, "%s: tensor %d has %lld elements", fn, i, (long long)numel[i]);
+        PSVAE_REQUIRE(numel[i] >= 0 && numel[i] <= (1ll << 40) && (total += numel[i]) <= (1ll << 40), PSVAE_EINVAL, "%s: tensor %d has %lld elements", fn, i, (long long)numel[i]);
         PSVAE_REQUIRE(types[i] == PSVAE_F32 || types[i] == PSVAE_BF16 || types[i] == PSVAE_F16, PSVAE_EINVAL, "%s: tensor %d is of an unknown type %d",
                       fn, i, (int)types[i]);
         PSVAE_REQUIRE(numel[i] == 0 || (grads[i] != nullptr && ((uintptr_t)grads[i] & (type_size(types[i]) - 1)) == 0), PSVAE_EINVAL,
@@ -192,6 +199,20 @@ int check_list(const char *fn, int n, const void *const *grads, const int64_t *n
 
 // Whether an output shares memory with another output, or with a gradient other than the one that it is.
 bool overlaps(int n, const void *const *grads, const int64_t *numel, const int32_t *types, void *const *out, const int32_t *out_types) {
+    // slices of one buffer in their order, the gradients elsewhere: no sorting
+    uintptr_t low = 0, high = 0;
+    bool simple = true;
+    for (int i = 0; i < n && simple; ++i) {
+        if (numel[i] == 0) continue;
+        const uintptr_t o = (uintptr_t)out[i];
+        if (high == 0) low = o;
+        simple = o >= high, high = o + (uintptr_t)numel[i] * type_size(out_types[i]);
+    }
+    for (int i = 0; i < n && simple; ++i) {
+        const uintptr_t g = (uintptr_t)grads[i];
+        simple = numel[i] == 0 || g >= high || g + (uintptr_t)numel[i] * type_size(types[i]) <= low;
+    }
+    if (simple) return false;
     struct Range {
         uintptr_t begin, end;
         bool out;
@@ -214,53 +235,62 @@ bool overlaps(int n, const void *const *grads, const int64_t *numel, const int32
     return false;
 }
 
-// The list's next part for one launch: tensors [at, ...), at most LIST that hold anything.  Returns where the next part begins.
-int fill(List *l, int at, int n, const void *const *grads, const int64_t *numel, const int32_t *types, void *const *out, const int32_t *out_types,
-         long long chunk) {
+int chunk_of(int n, const int64_t *numel, const int32_t *types) {
+    long long bytes = 0;
+    for (int i = 0; i < n; ++i) bytes += numel[i] * type_size(types[i]);
+    return bytes >= LARGE ? CHUNK_LARGE : CHUNK_SMALL;
+}
+
+// Tensors [at, n) into a launch's part, as many that hold anything as it has room for.  Returns where the next part begins.
+template <typename L>
+int fill(L *l, int at, int n, const void *const *grads, const int64_t *numel, const int32_t *types, void *const *out, const int32_t *out_types, int chunk) {
     l->n = 0, l->chunk = chunk, l->first[0] = 0;
-    for (; at < n && l->n < LIST; ++at) {
+    for (; at < n && l->n < L::ROOM; ++at) {
         if (numel[at] == 0) continue;
+        const long long each = chunk / type_size(types[at]), chunks = (numel[at] + each - 1) / each;
         const int k = l->n;
-        l->src[k] = grads[at], l->dst[k] = out ? out[at] : nullptr, l->numel[k] = numel[at];
-        l->st[k] = (uint8_t)types[at], l->dt[k] = out_types ? (uint8_t)out_types[at] : 0;
-        l->first[k + 1] = l->first[k] + (int)((numel[at] + chunk - 1) / chunk);
+        l->src[k] = grads[at];
+        if (out) l->dst[k] = out[at];
+        l->size[k] = (unsigned long long)numel[at] | (unsigned long long)types[at] << 60 | (unsigned long long)(out_types ? out_types[at] : 0) << 62;
+        l->first[k + 1] = l->first[k] + (int)chunks;
         l->n = k + 1;
     }
     return at;
 }
+template <typename L> int groups(const L &l) { return std::min(l.first[l.n], GROUPS); }
 
-// the partial sums of squares of the whole list
-int squares(const char *fn, int n, const void *const *grads, const int64_t *numel, const int32_t *types, const Cut &cut, double *partial, hipStream_t st) {
-    List l;
-    long long base = 0;
+// the launches that a norm's list takes at most, each with its partial sums
+int norm_parts(int n) { return (n + NormList::ROOM - 1) / NormList::ROOM; }
+
+// the partial sums of squares of the whole list; *n_partial: how many
+int squares(const char *fn, int n, const void *const *grads, const int64_t *numel, const int32_t *types, double *partial, int *n_partial, hipStream_t st) {
+    NormList l;
+    *n_partial = 0;
     for (int at = 0; at < n;) {
-        at = fill(&l, at, n, grads, numel, types, nullptr, nullptr, cut.chunk);
+        at = fill(&l, at, n, grads, numel, types, nullptr, nullptr, chunk_of(n, numel, types));
         if (l.n == 0) break;
-        hipLaunchKernelGGL(grad_squares_kernel, dim3((unsigned)l.first[l.n]), dim3(NT), 0, st, l, partial + base);
+        hipLaunchKernelGGL(grad_squares_kernel, dim3((unsigned)groups(l)), dim3(NT), 0, st, l, partial + *n_partial);
         PSVAE_CHECK_LAUNCH(fn);
-        base += l.first[l.n];
+        *n_partial += groups(l);
     }
     return PSVAE_OK;
 }
 
 }  // namespace
 
-extern "C" size_t psvae_grad_norm_workspace_bytes(int n, const int64_t *numel_host) {
-    if (n <= 0 || numel_host == nullptr) return 0;
-    return (size_t)cut_of(n, numel_host).chunks * sizeof(double);
-}
+extern "C" size_t psvae_grad_norm_workspace_bytes(int n) { return n <= 0 ? 0 : (size_t)norm_parts(n) * GROUPS * sizeof(double); }
 
 extern "C" int psvae_grad_norm(int n, const void *const *grads_host, const int64_t *numel_host, const int32_t *types_host, float *norm,
                                void *workspace, size_t workspace_bytes, void *stream) {
     const char *fn = "psvae_grad_norm";
     if (int rc = check_list(fn, n, grads_host, numel_host, types_host)) return rc;
     PSVAE_REQUIRE(norm != nullptr, PSVAE_EINVAL, "%s: null norm", fn);
-    const Cut cut = cut_of(n, numel_host);
-    PSVAE_REQUIRE(cut.chunks == 0 || (workspace != nullptr && workspace_bytes >= (size_t)cut.chunks * sizeof(double) && psvae_aligned16(workspace)),
+    PSVAE_REQUIRE(n == 0 || (workspace != nullptr && workspace_bytes >= psvae_grad_norm_workspace_bytes(n) && psvae_aligned16(workspace)),
                   PSVAE_EWORKSPACE, "%s: workspace too small or not 16-byte aligned", fn);
     hipStream_t st = (hipStream_t)stream;
-    if (int rc = squares(fn, n, grads_host, numel_host, types_host, cut, (double *)workspace, st)) return rc;
-    hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(NT), 0, st, (const double *)workspace, (int)cut.chunks, norm);
+    int n_partial = 0;
+    if (int rc = squares(fn, n, grads_host, numel_host, types_host, (double *)workspace, &n_partial, st)) return rc;
+    hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(NT), 0, st, (const double *)workspace, n_partial, norm);
     PSVAE_CHECK_LAUNCH(fn);
     return PSVAE_OK;
 }
@@ -280,26 +310,27 @@ extern "C" int psvae_clip_grads(int n, const void *const *grads_host, const int6
         PSVAE_REQUIRE(false, PSVAE_ETOOLARGE, "%s: out of host memory", fn);
     }
     PSVAE_REQUIRE(!shared, PSVAE_EINVAL, "%s: an output overlaps another output, or a gradient that it is not", fn);
-    const Cut cut = cut_of(n, numel_host);
-    PSVAE_REQUIRE(cut.chunks == 0 || (workspace != nullptr && workspace_bytes >= (size_t)cut.chunks * sizeof(double) && psvae_aligned16(workspace)),
+    PSVAE_REQUIRE(n == 0 || (workspace != nullptr && workspace_bytes >= psvae_grad_norm_workspace_bytes(n) && psvae_aligned16(workspace)),
                   PSVAE_EWORKSPACE, "%s: workspace too small or not 16-byte aligned", fn);
     hipStream_t st = (hipStream_t)stream;
     const double *partial = (const double *)workspace;
-    if (int rc = squares(fn, n, grads_host, numel_host, types_host, cut, (double *)workspace, st)) return rc;
-    if (cut.chunks == 0) {
+    int n_partial = 0;
+    if (int rc = squares(fn, n, grads_host, numel_host, types_host, (double *)workspace, &n_partial, st)) return rc;
+    if (n_partial == 0) {            // no elements
         hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(NT), 0, st, partial, 0, norm);
         PSVAE_CHECK_LAUNCH(fn);
         return PSVAE_OK;
     }
-    // the parts of the list in reverse, for the same reason as the chunks
+    // the parts of the list from its end, for the same reason as the chunks
+    const int chunk = chunk_of(n, numel_host, types_host);
     for (int end = n; end > 0;) {
         int begin = end, held = 0;
-        while (begin > 0 && held < LIST) held += numel_host[--begin] > 0;
-        List l;
-        fill(&l, begin, end, grads_host, numel_host, types_host, out_host, out_types_host, cut.chunk);
+        while (begin > 0 && held < ClipList::ROOM) held += numel_host[--begin] > 0;
+        ClipList l;
+        fill(&l, begin, end, grads_host, numel_host, types_host, out_host, out_types_host, chunk);
         end = begin;
         if (l.n == 0) continue;
-        hipLaunchKernelGGL(clip_grads_kernel, dim3((unsigned)l.first[l.n]), dim3(NT), 0, st, l, partial, (int)cut.chunks, max_norm, norm);
+        hipLaunchKernelGGL(clip_grads_kernel, dim3((unsigned)groups(l)), dim3(NT), 0, st, l, partial, n_partial, max_norm, norm);
         PSVAE_CHECK_LAUNCH(fn);
     }
     return PSVAE_OK;

@@ -797,7 +797,7 @@ Tensor grad_norm(at::TensorList grads) {
     const TensorList l = list_of(grads, grads[0].device(), fn);
     const int n = (int)grads.size();
     Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat).memory_format(std::nullopt));
-    const size_t nbytes = psvae_grad_norm_workspace_bytes(n, l.numel.data());
+    const size_t nbytes = psvae_grad_norm_workspace_bytes(n);
     Tensor hold = scratch(nbytes, norm);
     check(psvae_grad_norm(n, l.ptr.data(), l.numel.data(), l.types.data(), norm.data_ptr<float>(), hold.data_ptr(), nbytes, cur_stream(norm)), fn);
     return norm;
@@ -815,7 +815,7 @@ Tensor clip_grads(at::TensorList grads, double max_norm, at::TensorList out) {
                          (out[i].sizes() == grads[i].sizes() && out[i].strides() == grads[i].strides())), fn,
                     ": output ", i, " must have its gradient's number of elements, in the same order in memory");
     Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat).memory_format(std::nullopt));
-    const size_t nbytes = psvae_grad_norm_workspace_bytes(n, l.numel.data());
+    const size_t nbytes = psvae_grad_norm_workspace_bytes(n);
     Tensor hold = scratch(nbytes, norm);
     std::vector<void *> dst(n);
     for (int i = 0; i < n; ++i) dst[i] = const_cast<void *>(o.ptr[i]);

@@ -103,7 +103,7 @@ _SIGNATURES = {
     'psvae_shaped_log_prob_bwd': (_c_int, [_p, _p, _p, _p, _p, _c_i64, _p]),
     'psvae_shaped_draw_workspace_bytes': (_c_size, [_p]),
     'psvae_shaped_draw': (_c_int, [_p, _p, _c_i64, _c_i64, _p, _p, _p, _c_size, _p]),
-    'psvae_grad_norm_workspace_bytes': (_c_size, [_c_int, _p]),
+    'psvae_grad_norm_workspace_bytes': (_c_size, [_c_int]),
     'psvae_grad_norm': (_c_int, [_c_int, _p, _p, _p, _p, _p, _c_size, _p]),
     'psvae_clip_grads': (_c_int, [_c_int, _p, _p, _p, _p, _p, _c_f32, _p, _p, _c_size, _p]),
     'psvae_embed_trans_fwd': (_c_int, [_c_int, _c_int, _p, _p, _p, _c_int, _c_int, _c_int, _p, _p, _c_int, _p]),

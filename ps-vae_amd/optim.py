@@ -97,14 +97,12 @@ class FlatAdam(torch.optim.Optimizer):
             g.update({k: v for k, v in saved.items() if k != 'params'})
 
 
-@torch.no_grad()
 def grad_norm(grads):
     """2-norm (float32 scalar on the GPU) over a list of gradient tensors, each dense, of float32, bfloat16 or float16, on one
     device: squares and sums in 64 bits, the same bits for the same sizes and values.  Nothing is copied together; capturable."""
     return hip.grad_norm(list(grads))
 
 
-@torch.no_grad()
 def clip_grads(grads, max_norm, out=None):
     """Scales a list of gradient tensors (as grad_norm takes) by min(1, max_norm / (norm + 1e-6)), norm their common 2-norm, and
     returns the norm.  In place; or into `out`, one tensor per gradient with as many elements - the slices of a flat float32
@@ -113,10 +111,9 @@ def clip_grads(grads, max_norm, out=None):
     return hip.clip_grads(grads, float(max_norm), grads if out is None else list(out))
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters, max_norm):
     """torch.nn.utils.clip_grad_norm_(parameters, max_norm) (norm_type 2) on the GPU for parameters of any mix of float types: two
-    kernel launches up to 120 gradients, whatever their sizes."""
+    kernel launches up to 140 gradients, whatever their sizes."""
     parameters = [parameters] if torch.is_tensor(parameters) else list(parameters)
     grads = [p.grad for p in parameters if p.grad is not None]
     if not grads:

@@ -147,8 +147,7 @@ def test_rejected_gradient_lists(L):
         assert norm(ptrs, numel, types) == EINVAL, (ptrs, numel, types)
     assert norm([P], [3], [0], out=None) == EINVAL and norm([P], [3], [0], n=-1) == EINVAL
     assert norm([P], [3], [0], ws=None) == EWORKSPACE and norm([P], [3], [0], nbytes=7) == EWORKSPACE and norm([P], [3], [0], ws=P + 8) == EWORKSPACE
-    assert L.psvae_grad_norm_workspace_bytes(0, None) == 0
-    assert L.psvae_grad_norm_workspace_bytes(2, (ctypes.c_int64 * 2)(0, 4097)) == 2 * 8
+    assert L.psvae_grad_norm_workspace_bytes(0) == 0 and L.psvae_grad_norm_workspace_bytes(2) == L.psvae_grad_norm_workspace_bytes(200) > 0
 
     def clip(ptrs, numel, types, outs, out_types, max_norm=1.0, out=P, ws=P):
         a, b, c = lists(ptrs, numel, types)
