@@ -596,7 +596,7 @@ size_t psvae_grad_norm_workspace_bytes(int n);
 int psvae_grad_norm(int n, const void *const *grads_host, const int64_t *numel_host, const int32_t *types_host,
                     float *norm, void *workspace, size_t workspace_bytes, void *stream);
 int psvae_clip_grads(int n, const void *const *grads_host, const int64_t *numel_host, const int32_t *types_host,
-                     void *const *out_host, const int32_t *out_types_host, float max_norm, float *norm,
+                     void *const *out_host, const int32_t *out_types_host, double max_norm, float *norm,
                      void *workspace, size_t workspace_bytes, void *stream);
 
 

@@ -163,12 +163,12 @@ template <typename S> __device__ __forceinline__ void scale_to(const S *g, void 
 }
 
 // The chunks are taken from the list's end: what the norm read last is what the last-level cache still holds.
-__global__ __launch_bounds__(NT) void clip_grads_kernel(ClipList l, const double *__restrict__ partial, int n_partial, float max_norm,
+__global__ __launch_bounds__(NT) void clip_grads_kernel(ClipList l, const double *__restrict__ partial, int n_partial, double max_norm,
                                                         float *__restrict__ norm) {
     __shared__ double sh[NT / 64];
     const double v = sqrt(total_of(partial, n_partial, sh));
     if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)v;
-    const double q = (double)max_norm / (v + 1e-6);
+    const double q = max_norm / (v + 1e-6);
     const float coef = q > 1. ? 1.f : (float)q;   // (a NaN stays one, as torch.clamp keeps it)
     for (int c = l.first[l.n] - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x)
         with_chunk(l, c, [&](int i, int st, int dt, long long at, int n) {
@@ -296,13 +296,13 @@ extern "C" int psvae_grad_norm(int n, const void *const *grads_host, const int64
 }
 
 extern "C" int psvae_clip_grads(int n, const void *const *grads_host, const int64_t *numel_host, const int32_t *types_host,
-                                void *const *out_host, const int32_t *out_types_host, float max_norm, float *norm, void *workspace,
+                                void *const *out_host, const int32_t *out_types_host, double max_norm, float *norm, void *workspace,
                                 size_t workspace_bytes, void *stream) {
     const char *fn = "psvae_clip_grads";
     if (int rc = check_list(fn, n, grads_host, numel_host, types_host)) return rc;
     if (int rc = check_list(fn, n, (const void *const *)out_host, numel_host, out_types_host)) return rc;
     PSVAE_REQUIRE(norm != nullptr, PSVAE_EINVAL, "%s: null norm", fn);
-    PSVAE_REQUIRE(max_norm >= 0.f, PSVAE_EINVAL, "%s: max_norm must not be negative", fn);
+    PSVAE_REQUIRE(max_norm >= 0., PSVAE_EINVAL, "%s: max_norm must not be negative", fn);
     bool shared = false;
     try {
         shared = overlaps(n, grads_host, numel_host, types_host, out_host, out_types_host);

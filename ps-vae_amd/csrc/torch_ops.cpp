@@ -819,7 +819,7 @@ Tensor clip_grads(at::TensorList grads, double max_norm, at::TensorList out) {
     Tensor hold = scratch(nbytes, norm);
     std::vector<void *> dst(n);
     for (int i = 0; i < n; ++i) dst[i] = const_cast<void *>(o.ptr[i]);
-    check(psvae_clip_grads(n, l.ptr.data(), l.numel.data(), l.types.data(), dst.data(), o.types.data(), (float)max_norm,
+    check(psvae_clip_grads(n, l.ptr.data(), l.numel.data(), l.types.data(), dst.data(), o.types.data(), max_norm,
                            norm.data_ptr<float>(), hold.data_ptr(), nbytes, cur_stream(norm)), fn);
     for (const Tensor &t : out)
         if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();   // (written through its pointer)

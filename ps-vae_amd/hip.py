@@ -105,7 +105,7 @@ _SIGNATURES = {
     'psvae_shaped_draw': (_c_int, [_p, _p, _c_i64, _c_i64, _p, _p, _p, _c_size, _p]),
     'psvae_grad_norm_workspace_bytes': (_c_size, [_c_int]),
     'psvae_grad_norm': (_c_int, [_c_int, _p, _p, _p, _p, _p, _c_size, _p]),
-    'psvae_clip_grads': (_c_int, [_c_int, _p, _p, _p, _p, _p, _c_f32, _p, _p, _c_size, _p]),
+    'psvae_clip_grads': (_c_int, [_c_int, _p, _p, _p, _p, _p, _c_f64, _p, _p, _c_size, _p]),
     'psvae_embed_trans_fwd': (_c_int, [_c_int, _c_int, _p, _p, _p, _c_int, _c_int, _c_int, _p, _p, _c_int, _p]),
     'psvae_clip_adam_workspace_bytes': (_c_size, [_c_ll]),
     'psvae_clip_adam_step': (_c_int, [_c_ll, _p, _p, _p, _p, _c_f32, _c_f32] + [_c_f64] * 5 + [_c_int, _c_int, _p, _p, _c_size, _p]),

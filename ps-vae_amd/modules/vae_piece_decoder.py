@@ -263,9 +263,46 @@ class VAEPieceDecoder(nn.Module):
         order = kept[torch.argsort(conf[kept], descending=True, stable=True)]
         return idx, conf, etype.to(torch.int64), order.tolist()
 
+    def piece_masks(self, piece_atom_counts, max_atom_num=None):
+        """The sampling loop's rules as a mask table (ops.pack_allowed), one row for each number of atoms that a molecule has
+        so far, 0 .. rows - 1 (any more: the last row): never <pad>, no end token before the first piece, and - with
+        max_atom_num - only pieces that still fit."""
+        cnt = piece_atom_counts
+        have = torch.arange(2 if max_atom_num is None else max_atom_num + 1, device=cnt.device)[:, None]
+        allowed = torch.ones(have.shape[0], cnt.numel(), dtype=torch.bool, device=cnt.device)
+        if max_atom_num is not None:
+            allowed &= have + cnt[None, :] <= max_atom_num
+        end = self.tokenizer.end_idx()
+        allowed[:, end] = True
+        allowed[0, end] = False
+        allowed[:, self.tokenizer.pad_idx()] = False
+        return ops.pack_allowed(allowed)
+
+    def piece_log_prob(self, z_vecs, pieces, temperature=1.0, shaping=None, max_atom_num=None, piece_atom_counts=None):
+        """Log-probability of every piece of given sequences under the distribution that sample_pieces_batch draws from with the
+        same temperature and shaping - what a policy gradient on sampled molecules needs, differentiable in the latents and the
+        parameters.  pieces [B, S] int64 as in training: <s>, the pieces, the end token, then <pad>.  Returns [B, S - 1]
+        float32, 0 at padding."""
+        shaping = dict(shaping or {})
+        cnt = self.tokenizer.piece_atom_counts() if piece_atom_counts is None else piece_atom_counts
+        cnt = torch.as_tensor(cnt, dtype=torch.int32, device=pieces.device)
+        fit = shaping.pop('fit_atoms', False)
+        if fit and max_atom_num is None:
+            raise ValueError('fit_atoms needs max_atom_num')
+        masks = self.piece_masks(cnt, max_atom_num if fit else None)
+        gold = pieces[:, 1:].contiguous()
+        atoms = cnt[gold]
+        before = torch.cumsum(atoms, 1, dtype=torch.int32) - atoms
+        seen = torch.arange(gold.shape[1], dtype=torch.int32, device=gold.device).repeat(gold.shape[0], 1)
+        past = dict(history=gold, history_len=seen) if {'repetition', 'presence', 'frequency'} & shaping.keys() else {}
+        return ops.shaped_log_prob(self.piece_logits(z_vecs, pieces),
+                                   torch.where(gold == self.tokenizer.pad_idx(), torch.full_like(gold, -1), gold),
+                                   temperature=temperature, allowed=masks, state=before.clamp(max=masks.shape[0] - 1),
+                                   **past, **shaping)
+
     @torch.no_grad()
     def sample_pieces_batch(self, z, max_atom_num, temperature, uniforms=None, piece_atom_counts=None,
-                            generator=None):
+                            generator=None, shaping=None):
         """The piece sampling loop of `inference` (:134-158) for a batch of latents: every step
         is one GRU cell over all still-active molecules (two GEMMs + the fused gate kernel),
         the vocabulary projection, the pad / first-step end masks, softmax(logits / T) and one
@@ -274,7 +311,12 @@ class VAEPieceDecoder(nn.Module):
         [B, max_pos] in [0,1), drawn here when None).  A molecule stops after the end token,
         when its atom count exceeds max_atom_num or at max_pos pieces, and its last sampled
         piece is dropped (:154-158).  Returns (piece_ids [B, max_pos-ish] padded with pad_idx,
-        lengths [B])."""
+        lengths [B]).
+
+        shaping: what else is done to the logits before the draw (the reference does nothing): a dict of repetition,
+        presence, frequency (penalties for the pieces that a molecule already has) and bias, as ops.shape_logits takes
+        them, and fit_atoms=True: only pieces that keep the molecule within max_atom_num atoms, so that none is
+        sampled only to be dropped."""
         dev = self.W_mean.weight.device
         tok = self.tokenizer
         z = z.to(dev).float().reshape(-1, self.latent_dim)
@@ -302,12 +344,20 @@ class VAEPieceDecoder(nn.Module):
         atoms = torch.zeros(B, dtype=torch.int32, device=dev)
         active = torch.ones(B, dtype=torch.uint8, device=dev)
         cnt = cnt.to(torch.int32)
+        if shaping is not None:
+            shaping = dict(shaping)
+            if {'repetition', 'presence', 'frequency'} & shaping.keys():
+                shaping.update(history=out, history_len=length)
+            if shaping.pop('fit_atoms', False):
+                shaping.update(allowed=self.piece_masks(cnt, max_atom_num), state=atoms)
         for t in range(max_pos):
             emb = self.piece_embedding(cur).contiguous()
             hip.gemm(B, 3 * H, E, emb, E, 1, w_ih, 1, E, gi, 3 * H, bias=rnn.bias_ih_l0)
             hip.gemm(B, 3 * H, H, h, H, 1, w_hh, 1, H, gh, 3 * H, bias=rnn.bias_hh_l0)
             hip.gru_cell_fwd(gi, gh, h, h_next, gates)
             logits = run_linear(self.to_vocab, h_next)
+            if shaping is not None:
+                logits = ops.shape_logits(logits, **shaping)
             # pad / first-step end masks, softmax(logits / T), the draw and the state update: one kernel
             hip.piece_draw(logits, temperature, uniforms[:, t], pad, end, t == 0, cnt, max_atom_num, max_pos, active, atoms,
                            length, out[:, t], cur)
@@ -447,15 +497,15 @@ class VAEPieceDecoder(nn.Module):
                 'n_blocks': lengths, 'csr_in': csr_in}
 
     @torch.no_grad()
-    def inference_batch(self, z, max_atom_num, add_edge_th, temperature, uniforms=None, fragments=None):
+    def inference_batch(self, z, max_atom_num, add_edge_th, temperature, uniforms=None, fragments=None, shaping=None):
         """`inference` (:128-270) for a batch of latents without its RDKit calls: sample the
         pieces, expand them into fragment graphs, predict the links between all cross-fragment
         atom pairs, add bonds greedily under the valence / ring-size rules and keep the largest
         connected block.  Returns (molecules, aux): molecules[b] = {'atoms': [chemical-vocabulary
         index], 'bonds': [(begin, end, bond index)]} with the dropped atoms removed and the rest
         renumbered (what the reference hands to Chem.SanitizeMol / Kekulize at :272-273, which
-        stay with RDKit); aux holds the device-side intermediate results."""
-        piece_ids, lengths = self.sample_pieces_batch(z, max_atom_num, temperature, uniforms=uniforms)
+        stay with RDKit); aux holds the device-side intermediate results.  shaping: see sample_pieces_batch."""
+        piece_ids, lengths = self.sample_pieces_batch(z, max_atom_num, temperature, uniforms=uniforms, shaping=shaping)
         g = self.expand_pieces(piece_ids, lengths, fragments)
         dev = g['x'].device
         B = lengths.numel()

@@ -41,7 +41,7 @@ def check(grads, max_norm, out=None):
 
 
 SIZES = {'one': [1], 'small': [1, 2, 3, 4, 5, 7, 8, 9, 0, 63, 64, 65], 'chunks': [4095, 4096, 4097, 8192, 12289], 'model': [300 * 300, 300, 302 * 200, 302, 1] * 6,
-         'many': [17 * i % 301 for i in range(300)], 'exact': [5] * 120, 'over': [5] * 121, 'large': [3000001, 5, 2500000]}
+         'many': [17 * i % 301 for i in range(300)], 'exact': [5] * 140, 'over': [5] * 141, 'exact norm': [5] * 200, 'over norm': [5] * 201, 'three': [3] * 401, 'large': [3000001, 5, 2500000]}
 
 
 @pytest.mark.parametrize('mode', ['in place', 'flat f32', 'flat bf16'])
