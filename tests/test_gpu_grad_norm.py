@@ -86,6 +86,18 @@ def test_range():
     check([torch.zeros(10, device=d)], 1.0)
 
 
+def test_more_than_32_bits_of_elements():
+    from ps_vae_amd import optim
+    d = dev()
+    n = 2 ** 31 + 2 ** 20 + 3
+    g = torch.zeros(n, dtype=torch.bfloat16, device=d)
+    g[0], g[2 ** 31 + 5], g[-1] = 3., 4., 12.
+    assert float(optim.grad_norm([g])) == 13.0
+    assert float(optim.clip_grads([g], 1.3)) == 13.0
+    want = torch.tensor([0.3, 0.4, 1.2]).bfloat16().tolist()
+    assert [float(g[0]), float(g[2 ** 31 + 5]), float(g[-1])] == want and int(torch.count_nonzero(g)) == 3
+
+
 def test_not_finite():
     from ps_vae_amd import optim
     d = dev()

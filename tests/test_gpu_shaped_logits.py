@@ -439,6 +439,124 @@ def test_gradient_against_differences():
         assert (np.abs(got - want)[ok] <= w['d_tol'][ok, i] + 1e-7).all(), (i, got, want)
 
 
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+def test_a_run_is_the_row(dtype):
+    """Enough rows that a workgroup has a whole one: a lane adds up to V / 256 terms.  The sum's share of the tolerance is V / 256 + 12 additions and
+    the exponentials' 10 u in place of the 90 u above (which covers 80 additions)."""
+    from ps_vae_amd import ops
+    d = dev()
+    R, V, n = 1030, 30001, 5
+    more = (V / 256 + 12 + 10) * U
+    c = make(R, 1, V, 200, dtype, seed=5)
+    kw = on(c, d)
+    first = dict(logits=c['logits'][:n], tokens=c['tokens'][:n], uniforms=c['uniforms'][:n], g=c['g'][:n],
+                 kw={k: (v[:n] if k not in ('bias', 'allowed') else v) for k, v in c['kw'].items()})
+    w = expect(first)
+    x = c['logits'].to(d).requires_grad_(True)
+    lp = ops.shaped_log_prob(x, c['tokens'].to(d), **kw)
+    close(lp[:n], w['lp'], w['lp_tol'] + more, 'log_prob')
+    dx, = torch.autograd.grad(lp, x, c['g'].to(d))
+    close(dx[:n], w['d'], w['d_tol'] + more * np.abs(c['g'][:n].numpy())[:, None] * w['slope'] + half_step(x.dtype, w['d']), 'log_prob backward')
+    tok, _ = ops.shaped_draw(x.detach(), c['uniforms'].to(d), **kw)
+    for r in range(n):
+        t, _, gap = shaping_ref.draw_row(w['y'][r], float(c['uniforms'][r]))
+        assert int(tok[r]) == t or gap < 1e-12
+
+
+def test_offsets_past_32_bits():
+    """Logits of more than 2^31 elements: the last rows come out as they do alone."""
+    from ps_vae_amd import ops
+    d = dev()
+    R, V = 70000, 32003
+    x = torch.empty(R, V, dtype=torch.bfloat16, device=d)
+    x[-3:] = (torch.randn(3, V, generator=torch.Generator().manual_seed(1)) * 3).bfloat16().to(d)
+    x[:-3] = 0.
+    hist = torch.randint(0, V, (R, 20), generator=torch.Generator().manual_seed(2)).to(d)
+    tok = torch.randint(0, V, (R,), generator=torch.Generator().manual_seed(3)).to(d)
+    u = torch.rand(R, generator=torch.Generator().manual_seed(4)).to(d)
+    opt = dict(repetition=1.3, presence=0.1, temperature=0.7)
+    leaf = x[-3:].clone().requires_grad_(True)
+    y = ops.shape_logits(x, history=hist, **opt)
+    assert torch.equal(y[-3:], ops.shape_logits(leaf.detach(), history=hist[-3:], **opt)) and bool((y[0] <= 0).all())
+    del y
+    t, l = ops.shaped_draw(x, u, history=hist, **opt)
+    t1, l1 = ops.shaped_draw(leaf.detach(), u[-3:], history=hist[-3:], **opt)
+    assert torch.equal(t[-3:], t1) and torch.allclose(l[-3:], l1, rtol=4 * U, atol=1e-9)
+    x.requires_grad_(True)
+    lp = ops.shaped_log_prob(x, tok, history=hist, **opt)
+    dx, = torch.autograd.grad(lp, x, torch.ones_like(lp))
+    lp1 = ops.shaped_log_prob(leaf, tok[-3:], history=hist[-3:], **opt)
+    dx1, = torch.autograd.grad(lp1, leaf, torch.ones_like(lp1))
+    # another tiling adds the row's terms in another order: both sums are off by 90 u at most, one bfloat16 step where that tips a rounding
+    assert bool(((lp[-3:] - lp1).abs() <= 180 * U + 8 * U * lp1.abs()).all())
+    assert bool(((dx[-3:].float() - dx1.float()).abs() <= 2 ** -7 * dx1.float().abs() + 1e-30).all())
+
+
+def test_improbable_tokens():
+    """u = 0 takes the first token of positive probability, however small: its score is exact, also far below the smallest double's logarithm's
+    neighbourhood."""
+    from ps_vae_amd import ops
+    d = dev()
+    for V in (20, 900, 6000):
+        x = torch.zeros(3, V)
+        x[0, 0], x[1, 0], x[2, 0] = -500., -700., -740.     # 2^-721, 2^-1010, 2^-1068 of the rest (the last below the normal doubles)
+        tok, lp = ops.shaped_draw(x.to(d), torch.zeros(3, device=d))
+        assert tok.tolist() == [0, 0, 0]
+        want = torch.tensor([-500., -700., -740.], dtype=torch.float64) - np.log(V - 1.)
+        # the third weight has 6 bits left
+        assert bool(((lp.double().cpu() - want).abs() <= torch.tensor([1e-4, 1e-4, 2e-2])).all()), (V, lp)
+
+
+def test_through_the_c_abi():
+    """psvae_shaping as ctypes fills it: the same values as through the operator."""
+    import ctypes
+    from ps_vae_amd import hip, ops
+    d = dev()
+    for dims in (2, 3):
+        c = make(4, 1 if dims == 2 else 3, 77, 9, 'bf16', seed=2, bias=2, dims=dims, states=5)
+        kw = on(c, d)
+        x = c['logits'].to(d)
+        T = 1 if dims == 2 else 3
+        s = hip.Shaping(B=4, T=T, V=77, dtype=hip.BF16, logits=x.data_ptr(), ld_b=x.stride(0), ld_t=x.stride(1) if dims == 3 else 0,
+                        history=kw['history'].data_ptr(), ld_history=9, L=9, history_len=kw['history_len'].data_ptr(), len_per_row=int(dims == 3),
+                        repetition_rows=kw['repetition'].data_ptr(), presence_rows=kw['presence'].data_ptr(), frequency_rows=kw['frequency'].data_ptr(),
+                        temperature_rows=kw['temperature'].data_ptr(), repetition=1., temperature=1., bias=kw['bias'].data_ptr(), ld_bias=77,
+                        allowed=kw['allowed'].data_ptr(), ld_allowed=3, S=5, state=kw['state'].data_ptr(), state_per_row=int(dims == 3))
+        out = torch.empty_like(x)
+        assert hip.lib().psvae_shape_logits_fwd(ctypes.byref(s), hip.ptr(out), 77, hip._stream()) == 0
+        assert torch.equal(out, ops.shape_logits(x, **kw))
+        assert hip.lib().psvae_shape_logits_fwd(ctypes.byref(s), hip.ptr(x), 77, hip._stream()) == 0     # in place
+        assert torch.equal(out, x)
+
+
+def test_in_place_over_a_wide_row():
+    import ctypes
+    from ps_vae_amd import hip, ops
+    d = dev()
+    c = make(3, 1, 20011, 300, 'f32', seed=12, states=0)
+    kw = on(c, d)
+    x = c['logits'].to(d)
+    want = ops.shape_logits(x, **kw)
+    s = hip.Shaping(B=3, T=1, V=20011, dtype=hip.F32, logits=x.data_ptr(), ld_b=20011, history=kw['history'].data_ptr(), ld_history=300, L=300,
+                    history_len=kw['history_len'].data_ptr(), repetition_rows=kw['repetition'].data_ptr(), presence_rows=kw['presence'].data_ptr(),
+                    frequency_rows=kw['frequency'].data_ptr(), temperature_rows=kw['temperature'].data_ptr(), repetition=1., temperature=1.,
+                    bias=kw['bias'].data_ptr())
+    assert hip.lib().psvae_shape_logits_fwd(ctypes.byref(s), hip.ptr(x), 20011, hip._stream()) == 0
+    assert torch.equal(x, want)
+
+
+def test_history_of_extreme_ids():
+    """Ids at the ends of 64 bits are outside the vocabulary like any others."""
+    from ps_vae_amd import ops
+    d = dev()
+    lo, hi = -2 ** 63, 2 ** 63 - 1
+    for V in (70, 3001, 40001):
+        x = torch.randn(2, V, generator=torch.Generator().manual_seed(V)).to(d)
+        bad = torch.tensor([[lo, 7, hi, lo + 1, -1, V, 2 ** 32 + 7, lo + 7], [hi] * 8], device=d)
+        good = torch.tensor([[7], [-1]], device=d)
+        assert torch.equal(ops.shape_logits(x, history=bad, frequency=0.5), ops.shape_logits(x, history=good, frequency=0.5))
+
+
 def test_empty_calls():
     from ps_vae_amd import ops
     d = dev()
