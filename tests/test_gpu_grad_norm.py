@@ -86,6 +86,18 @@ def test_range():
     check([torch.zeros(10, device=d)], 1.0)
 
 
+def test_thousands_of_tensors():
+    """More partial sums than the scaling's workgroups add up by themselves."""
+    from ps_vae_amd import optim
+    d = dev()
+    flat = torch.randn(9000 * 5, generator=torch.Generator().manual_seed(0)).to(d)
+    norm = float(flat.double().pow(2).sum().sqrt())
+    want = flat.double() * (0.5 * norm / (norm + 1e-6))
+    assert abs(float(optim.clip_grads(list(flat.split(5)), 0.5 * norm)) - norm) <= 2 * U * norm
+    assert bool(((flat.double() - want).abs() <= 2 * U * want.abs()).all())        # the factor's rounding and the product's
+    assert abs(float(optim.grad_norm(list(flat.split(5)))) - 0.5 * norm) <= 4 * U * norm
+
+
 def test_more_than_32_bits_of_elements():
     from ps_vae_amd import optim
     d = dev()
