@@ -275,26 +275,28 @@ __device__ __forceinline__ double power_of_two(double z) {
     return ldexp(p, (int)n);
 }
 
-// -1080 in place of t where the bit is clear: its power of two is 0
+// A number in -1080 .. -1080.25 in place of t where the bit is clear: its power of two is 0.  (Only the upper word needs replacing.)
 __device__ __forceinline__ double or_nothing(int word, double t) {
     const unsigned long long x = (unsigned long long)__double_as_longlong(t);
-    const unsigned lo = (unsigned)x & (unsigned)word, hi = ((unsigned)(x >> 32) & (unsigned)word) | (0xc090e000u & ~(unsigned)word);
-    return __longlong_as_double((long long)(((unsigned long long)hi << 32) | lo));
+    const unsigned hi = ((unsigned)(x >> 32) & (unsigned)word) | (0xc090e000u & ~(unsigned)word);
+    return __longlong_as_double((long long)(((unsigned long long)hi << 32) | (unsigned)x));
 }
 
 // The weights 2^(z - m) of a wave's elements, z = v * scale (scale: log2 e over the temperature), 0 where `allow` has no bit.  fill(k, v) gives
 // the v of pack k, take(k, weights) gets its weights, more(f) calls f for further z of this lane.
-// Any m will do that leaves the sum in range and comes to the same for equal rows, so m is the largest of 64 elements, each lane's first - its
-// product with the scale then needs no rounding of its own - and the largest of all (exactly: equal z have to give equal weights,
-// however large they are) only where these allow nothing, are not small numbers, or turn out to be far below the others.
+// Any m will do that leaves the sum in range and comes to the same for equal rows, so m is the `guess` that the caller brings from the wave's
+// elements before; if that is no number, the largest of 64 elements, each lane's first - its product with the scale then needs no rounding of
+// its own; and the largest of all (exactly: equal z have to give equal weights, however large they are) only where these allow nothing, are not small
+// numbers, or turn out to be far from the others.
 struct Weights {
     double sum, m;                   // m: NaN if an allowed value is, +inf if one is, -inf if there is none
 };
 template <int K, int VEC, typename Fill, typename Take, typename More>
-__device__ __forceinline__ Weights weigh(const uint32_t (&allow)[K], double scale, Fill fill, Take take, More more) {
+__device__ __forceinline__ Weights weigh(const uint32_t (&allow)[K], double scale, double &guess, Fill fill, Take take, More more) {
     double v[VEC];
     fill(0, v);
-    double m = (double)wave_max(allow[0] & 1u ? (float)(v[0] * scale) : NEG), sum = __builtin_nan("");
+    if (!(fabs(guess) < 1e6)) guess = (double)wave_max(allow[0] & 1u ? (float)(v[0] * scale) : NEG);
+    double m = guess, sum = __builtin_nan("");
     bool bad = false;
     if (fabs(m) < 1e6) {
         sum = 0.;
@@ -313,7 +315,7 @@ __device__ __forceinline__ Weights weigh(const uint32_t (&allow)[K], double scal
         more([&](double z) { bad |= z != z, sum += power_of_two(z - m); });
         sum = wave_sum(sum);
     }
-    if (!(sum < 0x1p500)) {
+    if (!(sum < 0x1p500 && sum > 0x1p-500)) {
         double largest = NEG64;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
@@ -666,15 +668,23 @@ __device__ __forceinline__ void stores_done() {
 }
 
 // Streams through a run: `f(packs, element of the row that they begin at)` for every step of SPAN elements, the steps shared out to the
-// waves in turn; a step's loads are requested while the step before is worked on, the first before `prepare()` runs.
-template <typename P, typename T, typename Prepare, typename F>
+// waves in turn.  AHEAD: a step's loads are requested while the step before is worked on, the first before `prepare()` runs (shape of 256 rows
+// of 131072 bf16 62.5 us, 64.6 without); the draw's 64-bit work hides loads better with 4 waves on a SIMD than with 3 and their next
+// step in registers (114 against 144 registers, 44 against 48 us for 250 rows of 100003).
+template <typename P, bool AHEAD, typename T, typename Prepare, typename F>
 __device__ __forceinline__ void stream(const Args &a, const Place &at, const Row<T> &w, const T *from, Prepare prepare, F f) {
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), full = at.n / P::SPAN;
-    P one, two;
+    P one;
     int s = wave;
-    if (s < full) one.load(from, w, at.base + s * P::SPAN);
+    if (AHEAD && s < full) one.load(from, w, at.base + s * P::SPAN);
     prepare();
-    if (s < full) {
+    if constexpr (!AHEAD) {
+        for (; s < full; s += WAVES) {
+            one.load(from, w, at.base + s * P::SPAN);
+            f(one, at.base + s * P::SPAN);
+        }
+    } else if (s < full) {
+        P two;
         const int last = full - 1 - ((full - 1 - wave) & (WAVES - 1));   // (after the last step it is requested once more: no path without loads)
         for (;;) {
             two.load(from, w, at.base + std::min(s + WAVES, last) * P::SPAN);
@@ -713,7 +723,7 @@ template <typename T, int K, bool BIAS> __global__ __launch_bounds__(NT) void sh
     const Rule<float> rule(w, 1.f);
     Seen<float> seen(run_lds, a.run, a.L);
     T *row = out + at.r * ld_out;
-    stream<P>(a, at, w, w.x, [&] { if (a.history) look_back<true>(seen, w, rule, at.base, at.n); },
+    stream<P, true>(a, at, w, w.x, [&] { if (a.history) look_back<true>(seen, w, rule, at.base, at.n); },
                  [&](const P &p, int first) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
@@ -761,7 +771,7 @@ __global__ __launch_bounds__(NT) void shape_run_bwd_kernel(Args a, const T *__re
     const Rule<float> rule(w, 1.f);
     Seen<float> seen(run_lds, a.run, 0);                 // (bits alone)
     const int b = a.T == 1 ? at.r : (int)((unsigned)at.r / (unsigned)a.T), t = at.r - b * a.T;
-    stream<P>(a, at, w, g + b * ld_gb + t * ld_gt, [&] { if (a.history) look_back<false>(seen, w, rule, at.base, at.n); },
+    stream<P, true>(a, at, w, g + b * ld_gb + t * ld_gt, [&] { if (a.history) look_back<false>(seen, w, rule, at.base, at.n); },
                  [&](const P &p, int first) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
@@ -825,7 +835,7 @@ __global__ __launch_bounds__(NT) void log_prob_run_kernel(Args a, const int64_t 
     Seen<float> seen(run_lds, a.run, a.L);
     const int tok = token_of(tokens[at.r], a.V);
     float m = NEG, s = 0.f;          // of this lane's elements so far
-    stream<P>(a, at, w, w.x, [&] { if (a.history) look_back<true>(seen, w, rule, at.base, at.n); },
+    stream<P, true>(a, at, w, w.x, [&] { if (a.history) look_back<true>(seen, w, rule, at.base, at.n); },
                  [&](const P &p, int first) {
         float y[K][P::VEC], top = m;
 #pragma unroll
@@ -945,7 +955,7 @@ __global__ __launch_bounds__(NT) void log_prob_run_bwd_kernel(Args a, const int6
     Seen<float> seen(run_lds, a.run, a.L);
     const Slope slope(a, at.r, tokens, stats, g, rule);
     T *row = dx + at.r * ld_dx;
-    stream<P>(a, at, w, w.x, [&] { if (a.history) look_back<true>(seen, w, rule, at.base, at.n); },
+    stream<P, true>(a, at, w, w.x, [&] { if (a.history) look_back<true>(seen, w, rule, at.base, at.n); },
                  [&](const P &p, int first) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
@@ -971,7 +981,7 @@ __global__ __launch_bounds__(NT) void log_prob_run_bwd_kernel(Args a, const int6
 }
 
 // ---- draw.  Measured: 10000 rows of 302 f32 13.6 us (vector unit 76 % busy: 500 instructions a row, half of them 64-bit); 250 rows of
-// 100003 f16 with histories of up to 4000 47 us for the weights (35 instructions an element, 25 of them 64-bit: they alone are 26 us) and
+// 100003 f16 with histories of up to 4000 44 us for the weights (38 instructions an element, 25 of them 64-bit, about 5 cycles each: 30 us) and
 // 9 us for the pick.
 template <typename T, int N>
 __global__ __launch_bounds__(NT) void draw_rows_kernel(Args a, const float *__restrict__ uniforms, long long ld_u, int64_t empty,
@@ -983,7 +993,8 @@ __global__ __launch_bounds__(NT) void draw_rows_kernel(Args a, const float *__re
     double v[N], e[N];
     u.sums(rule, v);
     const uint32_t allow[1] = {u.allow};
-    const Weights all = weigh<1, N>(allow, rule.scale, [&](int, double (&to)[N]) {
+    double guess = NEG64;
+    const Weights all = weigh<1, N>(allow, rule.scale, guess, [&](int, double (&to)[N]) {
 #pragma unroll
         for (int j = 0; j < N; ++j) to[j] = v[j];
     }, [&](int, const double (&from)[N]) {
@@ -1009,7 +1020,8 @@ template <typename T, int K, bool BIAS> __global__ __launch_bounds__(NT) void dr
     const Rule<double> rule(w, LOG2E64);
     Seen<double> seen(run_lds, a.run, a.L);
     const int pieces = (a.V + P::SPAN - 1) / P::SPAN, lane = threadIdx.x & 63;
-    stream<P>(a, at, w, w.x, [&] { if (a.history) look_back<true>(seen, w, rule, at.base, at.n); },
+    double guess = NEG64;
+    stream<P, false>(a, at, w, w.x, [&] { if (a.history) look_back<true>(seen, w, rule, at.base, at.n); },
                  [&](const P &p, int first) {
         uint32_t allow[K];
 #pragma unroll
@@ -1022,7 +1034,7 @@ template <typename T, int K, bool BIAS> __global__ __launch_bounds__(NT) void dr
             const int word = (first - at.base) >> 5, next = word + P::SPAN / 32;
             u0 = seen.rank[word], u1 = next < (at.n + 31) >> 5 ? seen.rank[next] : seen.total;
         }
-        const Weights all = weigh<K, P::VEC>(allow, rule.scale, [&](int k, double (&v)[P::VEC]) { p.sums(k, v); }, [](int, auto &) {},
+        const Weights all = weigh<K, P::VEC>(allow, rule.scale, guess, [&](int k, double (&v)[P::VEC]) { p.sums(k, v); }, [](int, auto &) {},
                                              [&](auto f) {
             for (int u = u0 + lane; u < u1; u += 64) f(seen.value[u]);
         });
@@ -1146,10 +1158,11 @@ Cut cut_of(const psvae_shaping *s) {
         c.blocks = (R + WAVES - 1) / WAVES;
         return c;
     }
-    // The longest runs that leave 1024 workgroups, 4 for each compute unit (a run pays for its walk through the history once); down
+    // The longest runs that leave 960 workgroups, close to 4 for each compute unit (a run pays for its walk through the history once: 250 rows
+    // of 100003 in 4 runs each 44 us, in 5 47, in 8 51); down
     // to 2048 elements, in smaller steps, where rows are few.  A long history's list of seen ids has to fit LDS: at most 4096 of them.
     const int longest = s->history != nullptr && s->L > 4096 ? 4096 : RUN_MAX;
-    long long runs = std::max<long long>(psvae_cdiv(s->V, longest), std::min<long long>(psvae_cdiv(s->V, 2048), (1024 + R - 1) / std::max<long long>(R, 1)));
+    long long runs = std::max<long long>(psvae_cdiv(s->V, longest), std::min<long long>(psvae_cdiv(s->V, 2048), (960 + R - 1) / std::max<long long>(R, 1)));
     c.run = psvae_cdiv(psvae_cdiv(s->V, runs), 1024) * 1024;
     if (c.run < 2048) c.run = 2048;
     c.per_lane = c.run > 2048 ? 16 : 8;

@@ -492,6 +492,35 @@ def test_offsets_past_32_bits():
     assert bool(((dx[-3:].float() - dx1.float()).abs() <= 2 ** -7 * dx1.float().abs() + 1e-30).all())
 
 
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+def test_draw_over_unequal_levels(dtype):
+    """Stretches of 512 logits at levels far apart, nothing or the type's lowest value: what a wave weighs its elements against fits only some."""
+    from ps_vae_amd import ops
+    d = dev()
+    R, V = 250, 32003
+    t = {'f32': torch.float32, 'bf16': torch.bfloat16}[dtype]
+    gen = torch.Generator().manual_seed(8)
+    levels = torch.tensor([0., 0., -2000., -700., 900., 400., 2e6, float('-inf'), torch.finfo(t).min])
+    few = torch.randint(2, len(levels) + 1, (R, 1), generator=gen)             # how many of the levels a row has
+    at = (torch.rand(R, (V + 511) // 512, generator=gen) * few).long().clamp(max=len(levels) - 1)
+    x = (torch.randn(R, V, generator=gen) + levels[at].repeat_interleave(512, 1)[:, :V]).clamp(min=torch.finfo(t).min).to(t)
+    x[:, ::7] = torch.where(levels[at].repeat_interleave(512, 1)[:, :V][:, ::7] == float('-inf'), torch.tensor(float('-inf'), dtype=t), x[:, ::7])
+    allowed = torch.ones(2, V, dtype=torch.bool)
+    allowed[1, torch.randint(0, V, (V - 40,), generator=gen)] = False
+    state = torch.randint(-1, 2, (R,), generator=gen).int()
+    u = torch.rand(R, generator=gen)
+    tok, lp = ops.shaped_draw(x.to(d), u.to(d), allowed=ops.pack_allowed(allowed).to(d), state=state.to(d))
+    for r in range(0, R, 3):
+        y = x[r].double().numpy()
+        if int(state[r]) >= 0:
+            y = np.where(allowed[int(state[r])].numpy(), y, -np.inf)
+        want, want_lp, gap = shaping_ref.draw_row(y, float(u[r]))
+        # the running sum of 32003 doubles may be off by V half steps, 1.8e-12
+        assert int(tok[r]) == want or gap < 2e-12, r
+        if int(tok[r]) == want:
+            assert abs(float(lp[r]) - want_lp) <= U * abs(want_lp) + 2e-12, r
+
+
 def test_improbable_tokens():
     """u = 0 takes the first token of positive probability, however small: its score is exact, also far below the smallest double's logarithm's
     neighbourhood."""
