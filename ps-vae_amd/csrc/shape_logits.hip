@@ -579,6 +579,14 @@ template <typename C> struct Seen {
     }
     __device__ __forceinline__ uint16_t &id(int u) const { return small[BESIDE ? u : 4 * u + 2]; }
     __device__ __forceinline__ uint16_t &hit(int u) const { return small[BESIDE ? cap + u : 4 * u + 3]; }
+    // (once the list is finished, beside a float: what is left to ask about entry u)
+    __device__ __forceinline__ bool allowed(int u) const { return hit(u) & 1; }
+    __device__ __forceinline__ bool above_zero(int u) const { return hit(u) & 2; }
+    // the entries [x, y) of the run's elements [at, at + span), at and span multiples of 32
+    __device__ __forceinline__ int2 among(int at, int span, int n) const {
+        const int next = (at + span) >> 5;
+        return make_int2(rank[at >> 5], next < (n + 31) >> 5 ? rank[next] : total);
+    }
 };
 
 constexpr int RUN_MAX = 32768;       // ranks and ids fit 16 bits; 1024 words of bits, 4 for each thread
@@ -639,8 +647,11 @@ __device__ __forceinline__ void look_back(Seen<C> &seen, const Row<T> &w, const 
         __syncthreads();
         for (int u = tid; u < total; u += NT) {
             const int at = seen.id(u), i = base + at;
-            const C v = rule.penalised((C)(float)w.x[i], count[u * STEP]) + (w.bias ? (C)w.bias[i] : (C)0);
-            seen.value[u] = w.allows(i) ? scaled(v, rule.scale) : (C)NEG;
+            const float l = (float)w.x[i];
+            const bool allowed = w.allows(i);
+            const C v = rule.penalised((C)l, count[u * STEP]) + (w.bias ? (C)w.bias[i] : (C)0);
+            seen.value[u] = allowed ? scaled(v, rule.scale) : (C)NEG;
+            if (Seen<C>::BESIDE) seen.hit(u) = (uint16_t)((allowed ? 1 : 0) | (l > 0.f ? 2 : 0));
         }
         __syncthreads();
     }
@@ -661,15 +672,34 @@ template <int VEC, typename C> __device__ __forceinline__ uint32_t seen_bits(con
     return at < n ? (seen.bits[at >> 5] >> (at & 31)) & ((1u << VEC) - 1u) : 0u;
 }
 
-// Behind a stream of stores, before others of the workgroup write over some of them: the stores have arrived, for every wave.
-__device__ __forceinline__ void stores_done() {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-}
+// A step's results on their way out: where some of them are replaced (`any`, the same in every lane: by `replace(results of the step)`), the wave
+// takes them through LDS, so that whole lines are stored.  (Stores of the replaced elements alone, behind the step's, cost a
+// second write of their lines: 119 against 101 us for shape of 4000 rows of 32768 bf16 with histories of up to 500.)
+template <typename P, typename T> struct Stage {
+    T cell[WAVES][P::SPAN];
+    template <typename Packs, typename F> __device__ __forceinline__ void pass(Packs &out, bool any, F replace) {
+        if (!any) return;
+        constexpr int K = sizeof(out) / sizeof(out[0]);
+        T *mine = cell[threadIdx.x >> 6];
+        in_order();                  // (the step before has been read)
+#pragma unroll
+        for (int k = 0; k < K; ++k) *reinterpret_cast<uint4 *>(mine + P::at(k)) = __builtin_bit_cast(uint4, out[k]);
+        in_order();
+        replace(mine);
+        in_order();
+#pragma unroll
+        for (int k = 0; k < K; ++k) out[k] = __builtin_bit_cast(Pack<T>, *reinterpret_cast<uint4 *>(mine + P::at(k)));
+    }
+    // one wave's accesses to LDS take place in their order; the compiler keeps to it here
+    static __device__ __forceinline__ void in_order() {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+};
 
 // Streams through a run: `f(packs, element of the row that they begin at)` for every step of SPAN elements, the steps shared out to the
 // waves in turn.  AHEAD: a step's loads are requested while the step before is worked on, the first before `prepare()` runs (shape of 256 rows
-// of 131072 bf16 62.5 us, 64.6 without); the draw's 64-bit work hides loads better with 4 waves on a SIMD than with 3 and their next
+// of 131072 bf16: 2 us less of 64); the draw's 64-bit work hides loads better with 4 waves on a SIMD than with 3 and their next
 // step in registers (114 against 144 registers, 44 against 48 us for 250 rows of 100003).
 template <typename P, bool AHEAD, typename T, typename Prepare, typename F>
 __device__ __forceinline__ void stream(const Args &a, const Place &at, const Row<T> &w, const T *from, Prepare prepare, F f) {
@@ -705,8 +735,25 @@ __device__ __forceinline__ void stream(const Args &a, const Place &at, const Row
 
 extern __shared__ __align__(16) char run_lds[];
 
+// A row's token where it lies in the run: its value as if it had not been seen, requested before the stream.  (Looking for it among the elements
+// that stream past would cost 2 instructions for each of them.)
+struct Token {
+    int i;                           // the element of the row; -1: none in the run
+    float y;                         // -inf where the mask forbids it
+    template <typename T> __device__ __forceinline__ Token(int tok, const Place &at, const Row<T> &w, const Rule<float> &rule) {
+        const bool here = tok >= at.base && tok < at.base + at.n;
+        const int j = here ? tok : at.base;
+        float v = (float)w.x[j];
+        if (w.bias) v += w.bias[j];
+        i = here ? tok : -1, y = w.allows(j) ? scaled(v, rule.scale) : NEG;
+    }
+    __device__ __forceinline__ bool unseen(const Args &a, const Seen<float> &seen, const Place &at) const {
+        return i >= 0 && !(a.history && ((seen.bits[(i - at.base) >> 5] >> ((i - at.base) & 31)) & 1u));
+    }
+};
+
 // ---- shape.  Measured: rows of 302 f32, 25600 of them, 17.4 us forward and 21.0 backward (62 MB each way: 3.6 and 3.0 TB/s, bound by
-// the latency of a row's dependent loads); 256 rows of 131072 bf16 with a bias row each 62 us (272 MB: 4.4 TB/s, the rate of a copy is 4.7).
+// the latency of a row's dependent loads); 256 rows of 131072 bf16 with a bias row each 57 us (272 MB: 4.8 TB/s, the rate of a copy is 4.7).
 template <typename T, int N> __global__ __launch_bounds__(NT) void shape_rows_kernel(Args a, T *__restrict__ out, long long ld_out) {
     __shared__ typename Narrow<T, N>::Lds lds[WAVES];
     const Narrow<T, N> u(a, lds, (const T *)a.logits, a.ld_b, a.ld_t);
@@ -722,22 +769,28 @@ template <typename T, int K, bool BIAS> __global__ __launch_bounds__(NT) void sh
     const Row<T> w = row_of<T>(a, at.r);
     const Rule<float> rule(w, 1.f);
     Seen<float> seen(run_lds, a.run, a.L);
+    __shared__ __align__(16) Stage<P, T> stage;
     T *row = out + at.r * ld_out;
+    const int lane = threadIdx.x & 63;
     stream<P, true>(a, at, w, w.x, [&] { if (a.history) look_back<true>(seen, w, rule, at.base, at.n); },
                  [&](const P &p, int first) {
+        Pack<T> o[K];
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const int i = first + P::at(k);
             float v[P::VEC];
             p.raw(k, rule, v);
             p.masked(k, NEG, v);
-            store_pack(row + i, rounded<T>(v), a.V - i);
+            o[k] = rounded<T>(v);
         }
+        if (a.history) {
+            const int2 some = seen.among(first - at.base, P::SPAN, at.n);
+            stage.pass(o, __builtin_amdgcn_readfirstlane(some.y - some.x) != 0, [&](T *to) {
+                for (int u = some.x + lane; u < some.y; u += 64) to[at.base + seen.id(u) - first] = (T)seen.value[u];
+            });
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k) store_pack(row + first + P::at(k), o[k], a.V - first - P::at(k));
     });
-    if (a.history) {
-        stores_done();
-        for (int u = threadIdx.x; u < seen.total; u += NT) row[at.base + seen.id(u)] = (T)seen.value[u];
-    }
 }
 
 // dl = g dy/dl; the logits are read only where the sign of a seen token's decides.
@@ -792,10 +845,11 @@ __global__ __launch_bounds__(NT) void shape_run_bwd_kernel(Args a, const T *__re
     });
 }
 
-// ---- log_prob.  Measured, 4000 rows of 32768 bf16 with histories of up to 500: forward 85 us (262 MB: 3.1 TB/s; vector unit 73 % busy, 15
-// instructions an element of which the power of two takes four slots), backward 126 us (524 MB: 4.2 TB/s).  Streamed stores took the
-// backward from 163 to 128 us, reading the rows from the end 154 to 128.  Sums are 32-bit: a lane's at most 128 terms of a run in a chain (rescaled where its maximum grows), 6 levels over
-// the wave, 4 waves, then the row's runs: the relative error stays below (128 + 10 + runs) * 2^-24 and is far below it on average.
+// ---- log_prob.  Measured, 4000 rows of 32768 bf16 with histories of up to 500, a bias and masks: forward 84 us (262 MB; 50 us, 5.2 TB/s, with neither
+// bias nor history: the bias costs 15, its 4 bytes an element coming from L2, the look back 11), backward 101 us (524 MB: 5.2 TB/s).
+// Streamed stores took the backward from 163 to 128 us, reading the rows from the end 154 to 128, whole lines (Stage) 122 to 101.
+// Sums are 32-bit: a lane's at most 128 terms of a run in a chain (rescaled where its maximum grows), 6 levels over the wave, 4
+// waves, then the row's runs: the relative error stays below (128 + 10 + runs) * 2^-24 and is far below it on average.
 template <typename T, int N>
 __global__ __launch_bounds__(NT) void log_prob_rows_kernel(Args a, const int64_t *__restrict__ tokens, float *__restrict__ lp,
                                                            float2 *__restrict__ stats) {
@@ -834,6 +888,7 @@ __global__ __launch_bounds__(NT) void log_prob_run_kernel(Args a, const int64_t 
     const Rule<float> rule(w, 1.f);
     Seen<float> seen(run_lds, a.run, a.L);
     const int tok = token_of(tokens[at.r], a.V);
+    const Token token(tok, at, w, rule);
     float m = NEG, s = 0.f;          // of this lane's elements so far
     stream<P, true>(a, at, w, w.x, [&] { if (a.history) look_back<true>(seen, w, rule, at.base, at.n); },
                  [&](const P &p, int first) {
@@ -847,12 +902,6 @@ __global__ __launch_bounds__(NT) void log_prob_run_kernel(Args a, const int64_t 
             const uint32_t allow = p.allow[k] & ~left_out;
 #pragma unroll
             for (int j = 0; j < P::VEC; ++j) y[k][j] = select(bit_word(allow, j), y[k][j], NEG), top = fmaxf(top, y[k][j]);
-            const unsigned here = (unsigned)(tok - i);
-            if (here < (unsigned)P::VEC && !((left_out >> here) & 1u)) {
-#pragma unroll
-                for (int j = 0; j < P::VEC; ++j)
-                    if (j == (int)here) at_token = y[k][j];
-            }
         }
         const float from = reference_of(top);
         float sum = 0.f;
@@ -862,6 +911,7 @@ __global__ __launch_bounds__(NT) void log_prob_run_kernel(Args a, const int64_t 
             for (int j = 0; j < P::VEC; ++j) sum += exp_from(y[k][j], from);
         s = s * exp_from(m, from) + sum, m = top;
     });
+    if (threadIdx.x == 0 && token.unseen(a, seen, at)) at_token = token.y;
     if (a.history) {
         for (int u = threadIdx.x; u < seen.total; u += NT) {
             const float y = seen.value[u], top = fmaxf(m, y), from = reference_of(top);
@@ -954,30 +1004,43 @@ __global__ __launch_bounds__(NT) void log_prob_run_bwd_kernel(Args a, const int6
     const Rule<float> rule(w, 1.f);
     Seen<float> seen(run_lds, a.run, a.L);
     const Slope slope(a, at.r, tokens, stats, g, rule);
+    const Token token(slope.tok, at, w, rule);
+    const float above = rule.factor(1.f), below = rule.factor(-1.f);
+    const bool token_allowed = w.allows(token.i < 0 ? at.base : token.i);
+    __shared__ __align__(16) Stage<P, T> stage;
     T *row = dx + at.r * ld_dx;
+    const int lane = threadIdx.x & 63;
     stream<P, true>(a, at, w, w.x, [&] { if (a.history) look_back<true>(seen, w, rule, at.base, at.n); },
                  [&](const P &p, int first) {
+        Pack<T> o[K];
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const int i = first + P::at(k);
             float v[P::VEC];
             p.raw(k, rule, v);
-            slope.of(i, v);
             const uint32_t allow = slope.zero ? 0u : p.allow[k];
 #pragma unroll
-            for (int j = 0; j < P::VEC; ++j) v[j] = select(bit_word(allow, j), v[j], 0.f);
-            store_pack(row + i, rounded<T>(v), a.V - i);
+            for (int j = 0; j < P::VEC; ++j) v[j] = select(bit_word(allow, j), slope.others * exp_from(v[j], slope.from), 0.f);
+            o[k] = rounded<T>(v);
         }
+        const bool holds_token = (unsigned)(token.i - first) < (unsigned)P::SPAN;
+        int2 some = make_int2(0, 0);
+        if (a.history) some = seen.among(first - at.base, P::SPAN, at.n);
+        stage.pass(o, holds_token || __builtin_amdgcn_readfirstlane(some.y - some.x) != 0, [&](T *to) {
+            if (holds_token && lane == 0 && token.unseen(a, seen, at)) {
+                float v[1] = {token.y};
+                slope.of(token.i, v);
+                to[token.i - first] = (T)(slope.zero || !token_allowed ? 0.f : v[0]);
+            }
+            for (int u = some.x + lane; u < some.y; u += 64) {
+                const int i = at.base + seen.id(u);
+                float v[1] = {seen.value[u]};
+                slope.of(i, v);
+                to[i - first] = (T)(slope.zero || !seen.allowed(u) ? 0.f : v[0] * (seen.above_zero(u) ? above : below));
+            }
+        });
+#pragma unroll
+        for (int k = 0; k < K; ++k) store_pack(row + first + P::at(k), o[k], a.V - first - P::at(k));
     });
-    if (a.history) {
-        stores_done();
-        for (int u = threadIdx.x; u < seen.total; u += NT) {
-            const int i = at.base + seen.id(u);
-            float v[1] = {seen.value[u]};
-            slope.of(i, v);
-            row[i] = (T)(slope.zero || !w.allows(i) ? 0.f : v[0] * rule.factor((float)w.x[i]));
-        }
-    }
 }
 
 // ---- draw.  Measured: 10000 rows of 302 f32 13.6 us (vector unit 76 % busy: 500 instructions a row, half of them 64-bit); 250 rows of
@@ -1029,14 +1092,11 @@ template <typename T, int K, bool BIAS> __global__ __launch_bounds__(NT) void dr
             allow[k] = p.allow[k];
             if (a.history) allow[k] &= ~seen_bits<P::VEC>(seen, first + P::at(k) - at.base, at.n);
         }
-        int u0 = 0, u1 = 0;          // the list's entries of this step
-        if (a.history) {
-            const int word = (first - at.base) >> 5, next = word + P::SPAN / 32;
-            u0 = seen.rank[word], u1 = next < (at.n + 31) >> 5 ? seen.rank[next] : seen.total;
-        }
+        int2 some = make_int2(0, 0);  // the list's entries of this step
+        if (a.history) some = seen.among(first - at.base, P::SPAN, at.n);
         const Weights all = weigh<K, P::VEC>(allow, rule.scale, guess, [&](int k, double (&v)[P::VEC]) { p.sums(k, v); }, [](int, auto &) {},
                                              [&](auto f) {
-            for (int u = u0 + lane; u < u1; u += 64) f(seen.value[u]);
+            for (int u = some.x + lane; u < some.y; u += 64) f(seen.value[u]);
         });
         if (lane == 0) part[(long long)at.r * pieces + first / P::SPAN] = Piece{all.sum, all.m};
     });
