@@ -463,6 +463,36 @@ def test_a_run_is_the_row(dtype):
         assert int(tok[r]) == t or gap < 1e-12
 
 
+@pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('R,V,L', [(1000, 8195, 300), (970, 12290, 6000), (970, 6001, 6500)])
+def test_lines_with_seen_elements(R, V, L, dtype):
+    """Runs of many steps, each with elements of the history in most of its lines; histories longer than a run has room for."""
+    from ps_vae_amd import ops
+    d = dev()
+    n = 6
+    c = make(R, 1, V, L, dtype, seed=R + L, bias=2)
+    c['tokens'][:n // 2] = c['kw']['history'][:n // 2, -1].clamp(0, V - 1)          # half of the tokens seen, or likely to be
+    kw = on(c, d)
+    first = dict(logits=c['logits'][:n], tokens=c['tokens'][:n], g=c['g'][:n], kw={k: (v[:n] if k != 'allowed' else v) for k, v in c['kw'].items()})
+    w = expect(first)
+    x = c['logits'].to(d).requires_grad_(True)
+    y = ops.shape_logits(x, **kw)
+    close(y[:n], w['y'], w['y_tol'] + half_step(x.dtype, w['y']), 'shape')
+    gy = torch.randn(x.shape, generator=torch.Generator().manual_seed(1)).to(x.dtype)
+    dx, = torch.autograd.grad(y, x, gy.to(d))
+    want = gy[:n].double().numpy() * w['slope']
+    close(dx[:n], want, 4 * U * np.abs(want) + half_step(x.dtype, want), 'shape backward')
+    lp = ops.shaped_log_prob(x, c['tokens'].to(d), **kw)
+    close(lp[:n], w['lp'], w['lp_tol'], 'log_prob')
+    dx, = torch.autograd.grad(lp, x, c['g'].to(d))
+    close(dx[:n], w['d'], w['d_tol'] + half_step(x.dtype, w['d']), 'log_prob backward')
+    # the last row against a call of its own, whose runs are others
+    r = R - 1
+    one = c['logits'][r:].to(d).requires_grad_(True)
+    alone = {k: (v[r:] if k != 'allowed' else v) for k, v in kw.items()}
+    assert torch.equal(ops.shape_logits(one, **alone), y[r:])
+
+
 def test_offsets_past_32_bits():
     """Logits of more than 2^31 elements: the last rows come out as they do alone."""
     from ps_vae_amd import ops
