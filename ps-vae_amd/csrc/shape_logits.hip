@@ -698,9 +698,10 @@ template <typename P, typename T> struct Stage {
 };
 
 // Streams through a run: `f(packs, element of the row that they begin at)` for every step of SPAN elements, the steps shared out to the
-// waves in turn.  AHEAD: a step's loads are requested while the step before is worked on, the first before `prepare()` runs (shape of 256 rows
-// of 131072 bf16: 2 us less of 64); the draw's 64-bit work hides loads better with 4 waves on a SIMD than with 3 and their next
-// step in registers (114 against 144 registers, 44 against 48 us for 250 rows of 100003).
+// waves in turn.  AHEAD: a step's loads are requested while the step before is worked on, the first before `prepare()` runs.  Where
+// that costs waves of a SIMD it does not pay: the draw takes 114 registers without and 144 with it (44 against 48 us for 250 rows of 100003), the backward
+// of log_prob 56 and 82 (99.6 against 102.9 us for 4000 rows of 32768); shape has 76 with it (58 us for 256 rows of
+// 131072, 59 without; 142 and 138 for 4000 of 32768), the forward of log_prob 72 (no difference).
 template <typename P, bool AHEAD, typename T, typename Prepare, typename F>
 __device__ __forceinline__ void stream(const Args &a, const Place &at, const Row<T> &w, const T *from, Prepare prepare, F f) {
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), full = at.n / P::SPAN;
@@ -846,7 +847,7 @@ __global__ __launch_bounds__(NT) void shape_run_bwd_kernel(Args a, const T *__re
 }
 
 // ---- log_prob.  Measured, 4000 rows of 32768 bf16 with histories of up to 500, a bias and masks: forward 84 us (262 MB; 50 us, 5.2 TB/s, with neither
-// bias nor history: the bias costs 15, its 4 bytes an element coming from L2, the look back 11), backward 101 us (524 MB: 5.2 TB/s).
+// bias nor history: the bias costs 15, its 4 bytes an element coming from L2, the look back 11), backward 99.6 us (524 MB: 5.3 TB/s).
 // Streamed stores took the backward from 163 to 128 us, reading the rows from the end 154 to 128, whole lines (Stage) 122 to 101.
 // Sums are 32-bit: a lane's at most 128 terms of a run in a chain (rescaled where its maximum grows), 6 levels over the wave, 4
 // waves, then the row's runs: the relative error stays below (128 + 10 + runs) * 2^-24 and is far below it on average.
@@ -1010,7 +1011,7 @@ __global__ __launch_bounds__(NT) void log_prob_run_bwd_kernel(Args a, const int6
     __shared__ __align__(16) Stage<P, T> stage;
     T *row = dx + at.r * ld_dx;
     const int lane = threadIdx.x & 63;
-    stream<P, true>(a, at, w, w.x, [&] { if (a.history) look_back<true>(seen, w, rule, at.base, at.n); },
+    stream<P, false>(a, at, w, w.x, [&] { if (a.history) look_back<true>(seen, w, rule, at.base, at.n); },
                  [&](const P &p, int first) {
         Pack<T> o[K];
 #pragma unroll
