@@ -6,17 +6,17 @@
 //     log_prob = y_tok - m - log s,  m = max y, s = sum exp(y - m);  d log_prob / d l_i = ([i = tok] - exp(y_i - m) / s) dy_i/dl_i
 //     draw:  min(#{i : cdf_i <= u cdf_last}, last i of positive probability),  cdf the running sum of exp(y - m) in index order
 //
-// Bound: one read of the logits (and one write) at large sizes, launches at small ones, with 12 to 25 vector instructions an element in
-// between that have to stay under the time of the loads.
+// Bound: one read of the logits (and one write) at large sizes, launches at small ones, with 8 to 14 vector instructions an element in
+// between that have to stay under the time of the loads; the draw, whose 25 of 38 are 64-bit, is bound by them.
 //
 // Rows of at most 1024 logits: one wave each (Narrow).  Wider rows are cut into runs of up to 32768 elements, a workgroup each, whose
-// waves stream through it in steps of 512 or 1024 elements with the next step's loads in flight (Run).
+// waves stream through it in steps of 512 or 1024 elements (`stream`).
 //
 // The penalties need c_i.  No table of counts of [rows, V] is kept or read - it would be as large as the logits.  The
 // workgroup walks the row's history itself (8 bytes an entry) and builds in LDS what its elements need: one bit per element says whether the id was
 // seen, and the finished values y of the seen ids - computed once by one thread each - lie in a list in the order of the bits.  The
-// stream over the elements leaves the seen ones out of its sums, or writes them as if nothing had been seen; the list's values are added,
-// or written over these, afterwards.  So an element that was not seen, which nearly all are not, pays nothing for the question (looked up
+// stream over the elements leaves the seen ones out of its sums, the list's values being added beside it; or takes them as if nothing had been
+// seen, the list's values replacing these on their way out (Stage).  So an element that was not seen, which nearly all are not, pays nothing for the question (looked up
 // element by element the seen ones cost 8 of 24 instructions).  Counts are sums of integers and every value is computed from them
 // alone: the order of the LDS atomics does not show.
 #include "common.h"
