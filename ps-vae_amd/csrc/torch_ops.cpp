@@ -629,6 +629,13 @@ psvae_shaping shaping_of(const ShapingArgs &a, const char *fn) {
     "Tensor logits, Tensor? history, Tensor? history_len, Tensor? repetition, Tensor? presence, Tensor? frequency, " \
     "Tensor? temperature, float[] scalars, Tensor? bias, Tensor? allowed, Tensor? state"
 
+// No operator here has a forward-mode derivative: a tangent on an operand is an error, for the result would come back without one.
+void no_tangents(const char *fn, std::initializer_list<const Tensor *> operands) {
+    for (const Tensor *t : operands)
+        TORCH_CHECK(t == nullptr || !t->_fw_grad(0).defined(), fn, ": forward-mode derivatives are not implemented");
+}
+#define PSVAE_SHAPING_FLOATS p(logits), p(repetition), p(presence), p(frequency), p(temperature), p(bias)
+
 // Scratch of one call: a tensor of its own from the allocator (stream-ordered, and inside a captured graph's own pool), so
 // that no two graphs or streams ever meet in it.
 Tensor scratch(size_t nbytes, const Tensor &like) { return at::empty({(int64_t)nbytes}, like.options().dtype(at::kByte)); }
@@ -645,6 +652,7 @@ Tensor shape_logits_forward(PSVAE_SHAPING_PARAMS) {
 Tensor shape_logits_backward(const Tensor &g, PSVAE_SHAPING_PARAMS) {
     PSVAE_ON_DEVICE("psvae::shape_logits_backward", p(g), PSVAE_SHAPING_TENSORS);
     const char *fn = "psvae_shape_logits_bwd";
+    no_tangents(fn, {p(g)});
     const psvae_shaping s = shaping_of(PSVAE_SHAPING_ARGS, fn);
     TORCH_CHECK(g.sizes() == logits.sizes() && g.scalar_type() == logits.scalar_type(), fn, ": the gradient has the logits' shape and type");
     const Tensor gc = s.V == 1 || g.stride(-1) == 1 ? g : g.contiguous();
@@ -678,6 +686,7 @@ std::tuple<Tensor, Tensor> shaped_log_prob_forward(const Tensor &tokens, PSVAE_S
 Tensor shaped_log_prob_backward(const Tensor &g, const Tensor &stats, const Tensor &tokens, PSVAE_SHAPING_PARAMS) {
     PSVAE_ON_DEVICE("psvae::shaped_log_prob_backward", p(g), p(stats), p(tokens), PSVAE_SHAPING_TENSORS);
     const char *fn = "psvae_shaped_log_prob_bwd";
+    no_tangents(fn, {p(g)});
     const psvae_shaping s = shaping_of(PSVAE_SHAPING_ARGS, fn);
     const int64_t *tok = row_tokens(tokens, logits, fn);
     const int64_t rows = (int64_t)s.B * s.T;
@@ -692,6 +701,7 @@ Tensor shaped_log_prob_backward(const Tensor &g, const Tensor &stats, const Tens
 std::tuple<Tensor, Tensor> shaped_draw(const Tensor &uniforms, int64_t empty_token, PSVAE_SHAPING_PARAMS) {
     PSVAE_ON_DEVICE("psvae::shaped_draw", p(uniforms), PSVAE_SHAPING_TENSORS);
     const char *fn = "psvae_shaped_draw";
+    no_tangents(fn, {PSVAE_SHAPING_FLOATS});
     TORCH_CHECK(logits.dim() == 2, fn, ": logits must be [B, V]: one token per sequence is drawn");
     const psvae_shaping s = shaping_of(PSVAE_SHAPING_ARGS, fn);
     TORCH_CHECK(uniforms.dim() == 1 && uniforms.size(0) == logits.size(0), fn, ": uniforms must be [B]");
@@ -759,12 +769,14 @@ struct ShapedLogProb : torch::autograd::Function<ShapedLogProb> {
 bool wants_gradient(const Tensor &logits) { return at::GradMode::is_enabled() && logits.requires_grad(); }
 
 Tensor shape_logits(PSVAE_SHAPING_PARAMS) {
+    no_tangents("psvae_shape_logits", {PSVAE_SHAPING_FLOATS});
     if (wants_gradient(logits))
         return ShapeLogits::apply(logits, history, history_len, repetition, presence, frequency, temperature, scalars, bias, allowed, state);
     return shape_logits_forward(logits, history, history_len, repetition, presence, frequency, temperature, scalars, bias, allowed, state);
 }
 
 Tensor shaped_log_prob(const Tensor &tokens, PSVAE_SHAPING_PARAMS) {
+    no_tangents("psvae_shaped_log_prob", {PSVAE_SHAPING_FLOATS});
     if (wants_gradient(logits))
         return ShapedLogProb::apply(tokens, logits, history, history_len, repetition, presence, frequency, temperature, scalars, bias, allowed, state);
     return std::get<0>(shaped_log_prob_forward(tokens, logits, history, history_len, repetition, presence, frequency, temperature, scalars, bias,
@@ -783,6 +795,7 @@ TensorList list_of(at::TensorList ts, c10::Device device, const char *fn) {
     for (const Tensor &t : ts) {
         TORCH_CHECK(t.is_cuda(), fn, ": psvae operators need GPU tensors (there is no CPU fallback)");
         TORCH_CHECK(t.device() == device, fn, ": tensors on different devices (", device, " and ", t.device(), ")");
+        no_tangents(fn, {&t});
         TORCH_CHECK(t.layout() == at::kStrided && t.is_non_overlapping_and_dense(), fn,
                     ": a gradient must be dense, each of its elements in a place of its own");
         l.ptr.push_back(t.const_data_ptr()), l.numel.push_back(t.numel()), l.types.push_back(elem_type(t, fn));

@@ -1062,7 +1062,7 @@ def shape_logits(logits, *, history=None, history_len=None, repetition=None, pre
     allowed: a table of masks (pack_allowed); state int32 [B] or [B, T]: the table's row for each row of logits - negative: nothing is
     forbidden, past the table: everything is; None: the table has one row for all, or one per sequence.
 
-    Differentiable in the logits (once); masked places get no gradient and what they hold is never looked at."""
+    Differentiable in the logits (once, in reverse mode; a forward-mode tangent is an error); masked places get no gradient and what they hold is never looked at."""
     shaping = _shaping(history, history_len, repetition, presence, frequency, bias, allowed, state, temperature)
     return hip.shape_logits(logits, *shaping)
 
@@ -1071,7 +1071,7 @@ def shaped_log_prob(logits, tokens, *, history=None, history_len=None, repetitio
                     allowed=None, state=None, temperature=None):
     """log softmax(y)[token] in float32, y as shape_logits shapes it (same arguments; never written out): tokens int64 [B] or
     [B, T], one for each row.  A token outside the vocabulary: 0 and no gradient (padding).  A token that the mask forbids, or a row
-    that allows none: -inf (the latter without gradient).  Differentiable in the logits (once)."""
+    that allows none: -inf (the latter without gradient).  Differentiable in the logits as shape_logits is."""
     shaping = _shaping(history, history_len, repetition, presence, frequency, bias, allowed, state, temperature)
     return hip.shaped_log_prob(tokens, logits, *shaping)
 

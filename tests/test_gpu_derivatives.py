@@ -1,0 +1,81 @@
+"""The derivatives that the shaped logits and the gradient lists do not have: asking for one is an error, never a silent zero."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwAD
+
+pytestmark = pytest.mark.gpu
+
+
+def dev():
+    if not torch.cuda.is_available():
+        pytest.fail('GPU tests need a GPU')
+    return torch.device('cuda:0')
+
+
+def inputs(B=4, V=302):
+    g = torch.Generator().manual_seed(B * 1000 + V)
+    d = dev()
+    return dict(x=torch.randn(B, V, generator=g).to(d), tok=torch.randint(0, V, (B,), generator=g).to(d), u=torch.rand(B, generator=g).to(d),
+                h=torch.randint(0, V, (B, 9), generator=g).to(d), bias=torch.randn(V, generator=g).to(d), rows=(0.5 + torch.rand(B, generator=g)).to(d))
+
+
+def calls(c, **kw):
+    from ps_vae_amd import ops
+    return {'shape_logits': lambda x: ops.shape_logits(x, **kw), 'shaped_log_prob': lambda x: ops.shaped_log_prob(x, c['tok'], **kw),
+            'shaped_draw': lambda x: ops.shaped_draw(x, c['u'], **kw)}
+
+
+@pytest.mark.parametrize('needs_grad', [False, True])
+@pytest.mark.parametrize('V', [302, 5000])
+def test_forward_mode_of_the_logits_is_refused(V, needs_grad):
+    """A dual tensor came back without its tangent: a derivative that reads as zero."""
+    c = inputs(V=V)
+    for name, call in calls(c).items():
+        want = call(c['x'])
+        with fwAD.dual_level():
+            x = fwAD.make_dual(c['x'].clone().requires_grad_(needs_grad), torch.ones_like(c['x']))
+            with pytest.raises(RuntimeError, match='forward'):
+                call(x)
+            got = call(fwAD.unpack_dual(x).primal.detach())         # the values alone are fine
+        for a, b in zip(got if isinstance(got, tuple) else (got,), want if isinstance(want, tuple) else (want,)):
+            assert torch.equal(a, b), name
+
+
+def test_forward_mode_of_the_other_operands_is_refused():
+    c = inputs()
+    with fwAD.dual_level():
+        dual = lambda t: fwAD.make_dual(t, torch.ones_like(t))   # noqa: E731
+        for kw in (dict(bias=dual(c['bias'])), dict(temperature=dual(c['rows'])), dict(history=c['h'], repetition=dual(c['rows'])),
+                   dict(history=c['h'], presence=dual(c['rows'])), dict(history=c['h'], frequency=dual(c['rows']))):
+            for name, call in calls(c, **kw).items():
+                with pytest.raises(RuntimeError, match='forward'):
+                    call(c['x'])
+
+
+def test_forward_mode_over_the_backward_pass_is_refused():
+    """A tangent that only the incoming gradient has."""
+    from ps_vae_amd import ops
+    c = inputs()
+    for out in (lambda x: ops.shape_logits(x), lambda x: ops.shaped_log_prob(x, c['tok'])):
+        x = c['x'].clone().requires_grad_(True)
+        y = out(x)
+        g = torch.ones_like(y)
+        with fwAD.dual_level():
+            with pytest.raises(RuntimeError, match='forward'):
+                torch.autograd.grad(y, x, fwAD.make_dual(g, torch.ones_like(g)), retain_graph=True)
+        dx, = torch.autograd.grad(y, x, g)
+        assert bool(torch.isfinite(dx).all())
+
+
+def test_forward_mode_of_gradient_lists_is_refused():
+    from ps_vae_amd import optim
+    g = torch.ones(8, device=dev())
+    with fwAD.dual_level():
+        x = fwAD.make_dual(g, torch.ones_like(g))
+        with pytest.raises(RuntimeError, match='forward'):
+            optim.grad_norm([torch.ones(3, device=dev()), x])
+        with pytest.raises(RuntimeError, match='forward'):
+            optim.clip_grads([x], 1.0)
+        with pytest.raises(RuntimeError, match='forward'):
+            optim.clip_grads([g], 1.0, out=[fwAD.make_dual(torch.zeros(8, device=dev()), g)])
+    assert bool((g == 1).all())
