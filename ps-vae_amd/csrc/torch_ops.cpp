@@ -16,6 +16,7 @@
 #include <initializer_list>
 #include <map>
 #include <mutex>
+#include <string>
 #include <tuple>
 #include <utility>
 #include <vector>
@@ -698,6 +699,12 @@ Tensor shaped_log_prob_backward(const Tensor &g, const Tensor &stats, const Tens
     return out;
 }
 
+// The value alone, of something that autograd follows: a backward pass that comes here ends with `error` and not with a silent zero.
+Tensor end_of_graph(const Tensor &v, std::string error) {
+    return torch::autograd::DelayedError(std::move(error), 1)({v.detach().set_requires_grad(true)})[0];
+}
+bool wants_gradient(const Tensor &t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+
 std::tuple<Tensor, Tensor> shaped_draw(const Tensor &uniforms, int64_t empty_token, PSVAE_SHAPING_PARAMS) {
     PSVAE_ON_DEVICE("psvae::shaped_draw", p(uniforms), PSVAE_SHAPING_TENSORS);
     const char *fn = "psvae_shaped_draw";
@@ -712,6 +719,7 @@ std::tuple<Tensor, Tensor> shaped_draw(const Tensor &uniforms, int64_t empty_tok
     if (nbytes) hold = scratch(nbytes, logits);
     check(psvae_shaped_draw(&s, f32(uniforms, "uniforms"), uniforms.size(0) > 1 ? uniforms.stride(0) : 1, empty_token,
                             tokens.data_ptr<int64_t>(), lp.data_ptr<float>(), nbytes ? hold.data_ptr() : nullptr, nbytes, cur_stream(logits)), fn);
+    if (wants_gradient(logits)) lp = end_of_graph(lp, "psvae_shaped_draw: a draw has no backward pass (psvae::shaped_log_prob of the tokens has)");
     return {tokens, lp};
 }
 
@@ -725,9 +733,7 @@ OptTensor or_null(const Tensor &t) { return t.defined() ? OptTensor(t) : OptTens
 
 // Under create_graph a second backward pass would come through here: an error then, not a wrong constant.
 Tensor once(Tensor d, const char *fn) {
-    if (!at::GradMode::is_enabled()) return d;
-    d = d.detach().set_requires_grad(true);
-    return torch::autograd::DelayedError(std::string(fn) + ": the gradient cannot be differentiated again", 1)({d})[0];
+    return at::GradMode::is_enabled() ? end_of_graph(d, std::string(fn) + ": the gradient cannot be differentiated again") : d;
 }
 
 struct ShapeLogits : torch::autograd::Function<ShapeLogits> {
@@ -765,8 +771,6 @@ struct ShapedLogProb : torch::autograd::Function<ShapedLogProb> {
         return out;
     }
 };
-
-bool wants_gradient(const Tensor &logits) { return at::GradMode::is_enabled() && logits.requires_grad(); }
 
 Tensor shape_logits(PSVAE_SHAPING_PARAMS) {
     no_tangents("psvae_shape_logits", {PSVAE_SHAPING_FLOATS});

@@ -1081,6 +1081,6 @@ def shaped_draw(logits, uniforms, *, history=None, history_len=None, repetition=
     """One token per sequence from softmax(y) of logits [B, V], y as shape_logits shapes it: the first index whose running sum of
     probabilities exceeds uniforms[b] (float32 [B] in [0, 1)) times their total.  Returns (tokens int64 [B], log-probabilities
     float32 [B]).  A row that allows no token gives empty_token and -inf, one with NaN or +inf among its allowed values empty_token
-    and NaN."""
+    and NaN.  The log-probabilities are values: a backward pass through them is an error (shaped_log_prob of the tokens has one)."""
     shaping = _shaping(history, history_len, repetition, presence, frequency, bias, allowed, state, temperature)
     return hip.shaped_draw(uniforms, empty_token, logits, *shaping)

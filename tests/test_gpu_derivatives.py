@@ -79,3 +79,22 @@ def test_forward_mode_of_gradient_lists_is_refused():
         with pytest.raises(RuntimeError, match='forward'):
             optim.clip_grads([g], 1.0, out=[fwAD.make_dual(torch.zeros(8, device=dev()), g)])
     assert bool((g == 1).all())
+
+
+@pytest.mark.parametrize('V', [302, 5000])
+def test_drawn_log_probability_is_not_a_silent_constant(V):
+    """The draw has no backward pass: going back through its log-probability says so (it was a constant: a policy gradient of zero)."""
+    from ps_vae_amd import ops
+    c = inputs(V=V)
+    tok, lp = ops.shaped_draw(c['x'], c['u'])
+    assert not lp.requires_grad
+    x = c['x'].clone().requires_grad_(True)
+    tok1, lp1 = ops.shaped_draw(x, c['u'])
+    assert torch.equal(tok, tok1) and torch.equal(lp, lp1.detach()) and not tok1.requires_grad
+    with pytest.raises(RuntimeError, match='shaped_log_prob'):
+        (lp1.sum() + (x * x).sum()).backward()
+    with torch.no_grad():
+        assert not ops.shaped_draw(x, c['u'])[1].requires_grad
+    score = ops.shaped_log_prob(x, tok)                              # what takes its place
+    score.sum().backward()
+    assert bool(x.grad.any())
