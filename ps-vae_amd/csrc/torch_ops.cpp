@@ -13,6 +13,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <initializer_list>
 #include <map>
 #include <mutex>
@@ -704,6 +705,7 @@ Tensor end_of_graph(const Tensor &v, std::string error) {
     return torch::autograd::DelayedError(std::move(error), 1)({v.detach().set_requires_grad(true)})[0];
 }
 bool wants_gradient(const Tensor &t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+bool wants_gradient(at::TensorList ts) { return std::any_of(ts.begin(), ts.end(), [](const Tensor &t) { return wants_gradient(t); }); }
 
 std::tuple<Tensor, Tensor> shaped_draw(const Tensor &uniforms, int64_t empty_token, PSVAE_SHAPING_PARAMS) {
     PSVAE_ON_DEVICE("psvae::shaped_draw", p(uniforms), PSVAE_SHAPING_TENSORS);
@@ -817,12 +819,15 @@ Tensor grad_norm(at::TensorList grads) {
     const size_t nbytes = psvae_grad_norm_workspace_bytes(n);
     Tensor hold = scratch(nbytes, norm);
     check(psvae_grad_norm(n, l.ptr.data(), l.numel.data(), l.types.data(), norm.data_ptr<float>(), hold.data_ptr(), nbytes, cur_stream(norm)), fn);
-    return norm;
+    return wants_gradient(grads) ? end_of_graph(norm, "psvae_grad_norm: the norm cannot be differentiated") : norm;
 }
 
 Tensor clip_grads(at::TensorList grads, double max_norm, at::TensorList out) {
     const char *fn = "psvae_clip_grads";
     TORCH_CHECK(!grads.empty() && out.size() == grads.size(), fn, ": one output for each of at least one gradient");
+    // (written through its pointer, a leaf would change behind autograd's back and a result of a graph would keep its old derivative)
+    TORCH_CHECK(!wants_gradient(grads) && !wants_gradient(out), fn,
+                ": a tensor requires a gradient, and scaling cannot be differentiated: call it under torch.no_grad()");
     c10::DeviceGuard guard(same_device(fn, {&grads[0]}));
     const TensorList l = list_of(grads, grads[0].device(), fn), o = list_of(out, grads[0].device(), fn);
     const int n = (int)grads.size();

@@ -99,23 +99,26 @@ class FlatAdam(torch.optim.Optimizer):
 
 def grad_norm(grads):
     """2-norm (float32 scalar on the GPU) over a list of gradient tensors, each dense, of float32, bfloat16 or float16, on one
-    device: squares and sums in 64 bits, the same bits for the same sizes and values.  Nothing is copied together; capturable."""
+    device: squares and sums in 64 bits, the same bits for the same sizes and values.  Nothing is copied together; capturable.  Of gradients that
+    have a graph it is the value: a backward pass through it is an error."""
     return hip.grad_norm(list(grads))
 
 
 def clip_grads(grads, max_norm, out=None):
     """Scales a list of gradient tensors (as grad_norm takes) by min(1, max_norm / (norm + 1e-6)), norm their common 2-norm, and
     returns the norm.  In place; or into `out`, one tensor per gradient with as many elements - the slices of a flat float32
-    buffer, say, for gradients in bfloat16.  A norm that is not a number makes every gradient NaN, as torch's clip_grad_norm_ does."""
+    buffer, say, for gradients in bfloat16.  A norm that is not a number makes every gradient NaN, as torch's clip_grad_norm_ does.
+    Tensors that require a gradient are taken under torch.no_grad() alone."""
     grads = list(grads)
     return hip.clip_grads(grads, float(max_norm), grads if out is None else list(out))
 
 
 def clip_grad_norm_(parameters, max_norm):
     """torch.nn.utils.clip_grad_norm_(parameters, max_norm) (norm_type 2) on the GPU for parameters of any mix of float types: two
-    kernel launches up to 140 gradients, whatever their sizes."""
+    kernel launches up to 140 gradients, whatever their sizes.  As torch's, it takes gradients that have a graph for data."""
     parameters = [parameters] if torch.is_tensor(parameters) else list(parameters)
     grads = [p.grad for p in parameters if p.grad is not None]
     if not grads:
         return torch.zeros((), dtype=torch.float32, device=parameters[0].device if parameters else None)
-    return clip_grads(grads, max_norm)
+    with torch.no_grad():
+        return clip_grads(grads, max_norm)

@@ -98,3 +98,41 @@ def test_drawn_log_probability_is_not_a_silent_constant(V):
     score = ops.shaped_log_prob(x, tok)                              # what takes its place
     score.sum().backward()
     assert bool(x.grad.any())
+
+
+def test_norm_of_gradients_with_a_graph_is_not_a_silent_constant():
+    """A penalty on the norm contributed nothing."""
+    from ps_vae_amd import optim
+    d = dev()
+    w = torch.arange(1., 6., device=d, requires_grad=True)
+    g, = torch.autograd.grad((w ** 3).sum(), w, create_graph=True)
+    want = optim.grad_norm([g.detach()])
+    assert not want.requires_grad
+    norm = optim.grad_norm([torch.ones(0, device=d), g])
+    assert torch.equal(norm.detach(), want)
+    with pytest.raises(RuntimeError, match='grad_norm'):
+        (norm + w.sum()).backward()
+    with torch.no_grad():
+        assert torch.equal(optim.grad_norm([g]), want) and not optim.grad_norm([g]).requires_grad
+
+
+def test_clipping_what_autograd_follows_is_refused():
+    """Written through its pointer, a leaf would change under autograd, a graph's gradient would keep its old derivative."""
+    from ps_vae_amd import optim
+    d = dev()
+    w = torch.arange(1., 6., device=d, requires_grad=True)
+    g, = torch.autograd.grad((w ** 3).sum(), w, create_graph=True)
+    before, plain = g.detach().clone(), torch.ones(5, device=d)
+    for grads, out in (([g], None), ([w], None), ([plain], [w]), ([g], [plain]), ([plain, g], None)):
+        with pytest.raises(RuntimeError, match='no_grad'):
+            optim.clip_grads(grads, 1e-3, out=out)
+    assert torch.equal(g.detach(), before) and bool((plain == 1).all()) and w.detach().tolist() == [1., 2., 3., 4., 5.]
+    # under no_grad, and in clip_grad_norm_ as in torch's, a gradient with a graph is data
+    p = torch.nn.Parameter(torch.zeros(5, device=d))
+    p.grad = g
+    norm = optim.clip_grad_norm_([p], 1e-3)
+    assert not norm.requires_grad and abs(float(before.double().norm()) - float(norm)) <= 2 ** -23 * float(norm)
+    assert abs(float(g.detach().double().norm()) - 1e-3) < 1e-8
+    with torch.no_grad():
+        optim.clip_grads([g], 1e-4)
+    assert abs(float(g.detach().double().norm()) - 1e-4) < 1e-9
