@@ -133,6 +133,9 @@ def test_clipping_what_autograd_follows_is_refused():
     norm = optim.clip_grad_norm_([p], 1e-3)
     assert not norm.requires_grad and abs(float(before.double().norm()) - float(norm)) <= 2 ** -23 * float(norm)
     assert abs(float(g.detach().double().norm()) - 1e-3) < 1e-8
+    n = float(g.detach().double().norm())
     with torch.no_grad():
         optim.clip_grads([g], 1e-4)
-    assert abs(float(g.detach().double().norm()) - 1e-4) < 1e-9
+    # n 1e-4 / (n + 1e-6) with n = 1e-3 is 1e-4 / 1.001, a thousandth below 1e-4; the factor and each product are rounded once (2 * 2^-24 relative)
+    want = n * 1e-4 / (n + 1e-6)
+    assert abs(float(g.detach().double().norm()) - want) <= 2.01 * 2 ** -24 * want
