@@ -636,7 +636,17 @@ void no_tangents(const char *fn, std::initializer_list<const Tensor *> operands)
     for (const Tensor *t : operands)
         TORCH_CHECK(t == nullptr || !t->_fw_grad(0).defined(), fn, ": forward-mode derivatives are not implemented");
 }
-#define PSVAE_SHAPING_FLOATS p(logits), p(repetition), p(presence), p(frequency), p(temperature), p(bias)
+bool wants_gradient(const Tensor &t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+bool wants_gradient(at::TensorList ts) { return std::any_of(ts.begin(), ts.end(), [](const Tensor &t) { return wants_gradient(t); }); }
+
+// What is asked of a call's floating operands: only the logits have a gradient, in reverse mode.
+void check_operands(const char *fn, const Tensor &logits, std::initializer_list<const Tensor *> data) {
+    no_tangents(fn, {&logits});
+    no_tangents(fn, data);
+    for (const Tensor *t : data)
+        TORCH_CHECK(t == nullptr || !wants_gradient(*t), fn, ": penalties, temperature and bias are data: none of them gets a gradient");
+}
+#define PSVAE_CHECK_OPERANDS(fn) check_operands(fn, logits, {p(repetition), p(presence), p(frequency), p(temperature), p(bias)})
 
 // Scratch of one call: a tensor of its own from the allocator (stream-ordered, and inside a captured graph's own pool), so
 // that no two graphs or streams ever meet in it.
@@ -704,13 +714,11 @@ Tensor shaped_log_prob_backward(const Tensor &g, const Tensor &stats, const Tens
 Tensor end_of_graph(const Tensor &v, std::string error) {
     return torch::autograd::DelayedError(std::move(error), 1)({v.detach().set_requires_grad(true)})[0];
 }
-bool wants_gradient(const Tensor &t) { return at::GradMode::is_enabled() && t.requires_grad(); }
-bool wants_gradient(at::TensorList ts) { return std::any_of(ts.begin(), ts.end(), [](const Tensor &t) { return wants_gradient(t); }); }
 
 std::tuple<Tensor, Tensor> shaped_draw(const Tensor &uniforms, int64_t empty_token, PSVAE_SHAPING_PARAMS) {
     PSVAE_ON_DEVICE("psvae::shaped_draw", p(uniforms), PSVAE_SHAPING_TENSORS);
     const char *fn = "psvae_shaped_draw";
-    no_tangents(fn, {PSVAE_SHAPING_FLOATS});
+    PSVAE_CHECK_OPERANDS(fn);
     TORCH_CHECK(logits.dim() == 2, fn, ": logits must be [B, V]: one token per sequence is drawn");
     const psvae_shaping s = shaping_of(PSVAE_SHAPING_ARGS, fn);
     TORCH_CHECK(uniforms.dim() == 1 && uniforms.size(0) == logits.size(0), fn, ": uniforms must be [B]");
@@ -775,14 +783,14 @@ struct ShapedLogProb : torch::autograd::Function<ShapedLogProb> {
 };
 
 Tensor shape_logits(PSVAE_SHAPING_PARAMS) {
-    no_tangents("psvae_shape_logits", {PSVAE_SHAPING_FLOATS});
+    PSVAE_CHECK_OPERANDS("psvae_shape_logits");
     if (wants_gradient(logits))
         return ShapeLogits::apply(logits, history, history_len, repetition, presence, frequency, temperature, scalars, bias, allowed, state);
     return shape_logits_forward(logits, history, history_len, repetition, presence, frequency, temperature, scalars, bias, allowed, state);
 }
 
 Tensor shaped_log_prob(const Tensor &tokens, PSVAE_SHAPING_PARAMS) {
-    no_tangents("psvae_shaped_log_prob", {PSVAE_SHAPING_FLOATS});
+    PSVAE_CHECK_OPERANDS("psvae_shaped_log_prob");
     if (wants_gradient(logits))
         return ShapedLogProb::apply(tokens, logits, history, history_len, repetition, presence, frequency, temperature, scalars, bias, allowed, state);
     return std::get<0>(shaped_log_prob_forward(tokens, logits, history, history_len, repetition, presence, frequency, temperature, scalars, bias,

@@ -1029,7 +1029,7 @@ def _number_or_rows(v, neutral):
     if v is None:
         return None, neutral
     if torch.is_tensor(v):
-        if v.requires_grad:
+        if v.requires_grad and torch.is_grad_enabled():
             raise ValueError('penalties and temperature are data: none of them gets a gradient')
         return v, neutral
     return None, float(v)
@@ -1039,7 +1039,7 @@ def _shaping(history, history_len, repetition, presence, frequency, bias, allowe
     """The operators' arguments behind the logits, in the order of torch.ops.psvae.shape_logits."""
     if history is None and not (repetition is None and presence is None and frequency is None):
         raise ValueError('penalties need a history')
-    if bias is not None and bias.requires_grad:
+    if bias is not None and bias.requires_grad and torch.is_grad_enabled():
         raise ValueError('the bias is data: it gets no gradient')
     repetition, r = _number_or_rows(repetition, 1.0)
     presence, p = _number_or_rows(presence, 0.0)
@@ -1062,7 +1062,8 @@ def shape_logits(logits, *, history=None, history_len=None, repetition=None, pre
     allowed: a table of masks (pack_allowed); state int32 [B] or [B, T]: the table's row for each row of logits - negative: nothing is
     forbidden, past the table: everything is; None: the table has one row for all, or one per sequence.
 
-    Differentiable in the logits (once, in reverse mode; a forward-mode tangent is an error); masked places get no gradient and what they hold is never looked at."""
+    Differentiable in the logits (once, in reverse mode; a forward-mode tangent is an error); masked places get no gradient and what they hold is never looked at.  The other operands are data: one that requires a
+    gradient is refused while gradients are recorded."""
     shaping = _shaping(history, history_len, repetition, presence, frequency, bias, allowed, state, temperature)
     return hip.shape_logits(logits, *shaping)
 

@@ -139,3 +139,32 @@ def test_clipping_what_autograd_follows_is_refused():
     # n 1e-4 / (n + 1e-6) with n = 1e-3 is 1e-4 / 1.001, a thousandth below 1e-4; the factor and each product are rounded once (2 * 2^-24 relative)
     want = n * 1e-4 / (n + 1e-6)
     assert abs(float(g.detach().double().norm()) - want) <= 2.01 * 2 ** -24 * want
+
+
+def test_data_operands_that_want_a_gradient():
+    """Refused where a gradient is being recorded, whichever way the operator is called; data like any other where none is."""
+    from ps_vae_amd import hip, ops
+    c = inputs()
+    raw = hip.ops()
+    for at, t in ((2, c['rows']), (3, c['rows']), (4, c['rows']), (5, c['rows']), (7, c['bias'])):
+        for x in (c['x'], c['x'].clone().requires_grad_(True)):
+            # history, its lengths, repetition, presence, frequency, temperature, their numbers, bias, allowed, state
+            args = [c['h'], None, None, None, None, None, [1., 0., 0., 1.], None, None, None]
+            args[at] = t.clone().requires_grad_(True)
+            for call in (lambda: raw.shape_logits(x, *args), lambda: raw.shaped_log_prob(c['tok'], x, *args),
+                         lambda: raw.shaped_draw(c['u'], -1, x, *args)):
+                with pytest.raises(RuntimeError, match='none of them gets a gradient'):
+                    call()
+                with torch.no_grad():
+                    call()
+    for key, t in (('bias', c['bias']), ('temperature', c['rows'])):
+        learned, plain = calls(c, **{key: torch.nn.Parameter(t)}), calls(c, **{key: t})
+        for name in plain:
+            with pytest.raises(ValueError, match='gradient'):
+                learned[name](c['x'])
+            with torch.no_grad():
+                got, want = learned[name](c['x']), plain[name](c['x'])
+            for a, b in zip(got if isinstance(got, tuple) else (got,), want if isinstance(want, tuple) else (want,)):
+                assert torch.equal(a, b), name
+    with torch.no_grad():
+        assert torch.equal(ops.shape_logits(c['x'], bias=torch.nn.Parameter(c['bias'])), ops.shape_logits(c['x'], bias=c['bias']))
