@@ -533,8 +533,10 @@ int psvae_piece_draw(int B, int V, const float *logits, int64_t ld_logits, float
  *                                     - frequency_b c_i - presence_b
  *   y_i = (a_i + bias_i) / temperature_b  where bit i of the row's mask is set, else -inf
  * Ids of the history outside 0 .. V-1 count for nothing.  What a masked logit holds (NaN,
- * infinities) is never looked at.  A repetition or temperature read from the device that is not positive
- * and finite makes the values that it touches NaN.
+ * infinities) is never looked at.  repetition and temperature lie in 2^-126 .. 2^126 (their reciprocals
+ * are normal numbers): one given as a number is checked, one read from the device that does not makes
+ * the values that it touches NaN.  shape_logits and log_prob form y in 32 bits (a y past float32's range
+ * is infinite, and a row that allows +inf has no log-probability: NaN), the draw in 64.
  * The mask row is allowed[s] with s = state[r or b]; s < 0: every token, s >= S: none; without
  * states row 0 (S == 1) or row b (S == B).  Bit i is bit i % 32 of word i / 32.
  * ---------------------------------------------------------------------------------- */

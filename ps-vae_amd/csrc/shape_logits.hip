@@ -72,7 +72,10 @@ template <typename T> struct Row {
     __device__ __forceinline__ bool allows(int i) const { return !none && (!mask || ((mask[i >> 5] >> (i & 31)) & 1u)); }
 };
 
-__device__ __forceinline__ float positive(float v) { return v > 0.f && v < __builtin_inff() ? v : __builtin_nanf(""); }
+// Repetition and temperature: numbers whose 32-bit reciprocal is a normal number too (beyond, the unit's estimate of it is infinite, or 0).
+constexpr float RULE_MIN = 0x1p-126f, RULE_MAX = 0x1p126f;
+__device__ __forceinline__ float in_range(float v) { return v >= RULE_MIN && v <= RULE_MAX ? v : __builtin_nanf(""); }
+bool is_in_range(float v) { return v >= RULE_MIN && v <= RULE_MAX; }
 
 template <typename T> __device__ __forceinline__ Row<T> row_of(const Args &a, int r) {
     const int b = a.T == 1 ? r : (int)((unsigned)r / (unsigned)a.T), t = r - b * a.T;
@@ -84,11 +87,11 @@ template <typename T> __device__ __forceinline__ Row<T> row_of(const Args &a, in
         const int n = a.history_len ? a.history_len[a.len_per_row ? r : b] : a.L;
         w.len = n < 0 ? 0 : (n < a.L ? n : a.L);
     }
-    // a repetition or temperature that is not a positive finite number makes what it touches NaN
-    w.rep = positive(a.rep_p ? a.rep_p[b] : a.rep);
+    // a repetition or temperature out of range makes what it touches NaN
+    w.rep = in_range(a.rep_p ? a.rep_p[b] : a.rep);
     w.pres = a.pres_p ? a.pres_p[b] : a.pres;
     w.freq = a.freq_p ? a.freq_p[b] : a.freq;
-    w.temp = positive(a.temp_p ? a.temp_p[b] : a.temp);
+    w.temp = in_range(a.temp_p ? a.temp_p[b] : a.temp);
     w.bias = a.bias ? a.bias + b * a.ld_bias : nullptr;
     w.mask = nullptr, w.none = false;
     if (a.allowed) {
@@ -1241,8 +1244,8 @@ int check_shaping(const char *fn, const psvae_shaping *s, Args *a) {
                   s->V);
     PSVAE_REQUIRE(cut_of(s).blocks <= MAX_BLOCKS, PSVAE_ETOOLARGE, "%s: %d x %d rows of %d are more than one launch holds", fn, s->B, s->T,
                   s->V);
-    PSVAE_REQUIRE(s->repetition > 0.f && s->repetition < __builtin_inff() && s->temperature > 0.f && s->temperature < __builtin_inff(),
-                  PSVAE_EINVAL, "%s: repetition and temperature must be positive and finite", fn);
+    PSVAE_REQUIRE(is_in_range(s->repetition) && is_in_range(s->temperature), PSVAE_EINVAL,
+                  "%s: repetition and temperature must lie in 2^-126 .. 2^126", fn);
     PSVAE_REQUIRE(s->presence - s->presence == 0.f && s->frequency - s->frequency == 0.f, PSVAE_EINVAL,
                   "%s: presence and frequency must be finite", fn);
     if (s->B == 0) return PSVAE_OK;
