@@ -263,19 +263,23 @@ class VAEPieceDecoder(nn.Module):
         order = kept[torch.argsort(conf[kept], descending=True, stable=True)]
         return idx, conf, etype.to(torch.int64), order.tolist()
 
-    def piece_masks(self, piece_atom_counts, max_atom_num=None):
-        """The sampling loop's rules as a mask table (ops.pack_allowed), one row for each number of atoms that a molecule has
-        so far, 0 .. rows - 1 (any more: the last row): never <pad>, no end token before the first piece, and - with
-        max_atom_num - only pieces that still fit."""
+    def _atoms_allowed(self, piece_atom_counts, max_atom_num=None):
+        """bool [atoms so far, vocabulary]: what may follow a piece - never <pad>, and with max_atom_num only pieces that still fit."""
         cnt = piece_atom_counts
         have = torch.arange(2 if max_atom_num is None else max_atom_num + 1, device=cnt.device)[:, None]
         allowed = torch.ones(have.shape[0], cnt.numel(), dtype=torch.bool, device=cnt.device)
         if max_atom_num is not None:
             allowed &= have + cnt[None, :] <= max_atom_num
-        end = self.tokenizer.end_idx()
-        allowed[:, end] = True
-        allowed[0, end] = False
+        allowed[:, self.tokenizer.end_idx()] = True
         allowed[:, self.tokenizer.pad_idx()] = False
+        return allowed
+
+    def piece_masks(self, piece_atom_counts, max_atom_num=None):
+        """The sampling loop's rules as a mask table (ops.pack_allowed), one row for each number of atoms that a molecule has
+        so far, 0 .. rows - 1 (any more: the last row): never <pad>, no end token before the first piece, and - with
+        max_atom_num - only pieces that still fit."""
+        allowed = self._atoms_allowed(piece_atom_counts, max_atom_num)
+        allowed[0, self.tokenizer.end_idx()] = False
         return ops.pack_allowed(allowed)
 
     def piece_log_prob(self, z_vecs, pieces, temperature=1.0, shaping=None, max_atom_num=None, piece_atom_counts=None):
@@ -289,15 +293,20 @@ class VAEPieceDecoder(nn.Module):
         fit = shaping.pop('fit_atoms', False)
         if fit and max_atom_num is None:
             raise ValueError('fit_atoms needs max_atom_num')
-        masks = self.piece_masks(cnt, max_atom_num if fit else None)
+        # row 0 is the first position's; behind the rows for the numbers of atoms one for none at a later position (after pieces without atoms)
+        allowed = self._atoms_allowed(cnt, max_atom_num if fit else None)
+        last, later = allowed.shape[0] - 1, allowed[:1].clone()
+        allowed[0, self.tokenizer.end_idx()] = False
+        masks = ops.pack_allowed(torch.cat([allowed, later]))
         gold = pieces[:, 1:].contiguous()
         atoms = cnt[gold]
-        before = torch.cumsum(atoms, 1, dtype=torch.int32) - atoms
+        state = (torch.cumsum(atoms, 1, dtype=torch.int32) - atoms).clamp(max=last)
+        state[:, 1:] = torch.where(state[:, 1:] == 0, last + 1, state[:, 1:])
         seen = torch.arange(gold.shape[1], dtype=torch.int32, device=gold.device).repeat(gold.shape[0], 1)
         past = dict(history=gold, history_len=seen) if {'repetition', 'presence', 'frequency'} & shaping.keys() else {}
         return ops.shaped_log_prob(self.piece_logits(z_vecs, pieces),
                                    torch.where(gold == self.tokenizer.pad_idx(), torch.full_like(gold, -1), gold),
-                                   temperature=temperature, allowed=masks, state=before.clamp(max=masks.shape[0] - 1),
+                                   temperature=temperature, allowed=masks, state=state,
                                    **past, **shaping)
 
     @torch.no_grad()
@@ -349,7 +358,8 @@ class VAEPieceDecoder(nn.Module):
             if {'repetition', 'presence', 'frequency'} & shaping.keys():
                 shaping.update(history=out, history_len=length)
             if shaping.pop('fit_atoms', False):
-                shaping.update(allowed=self.piece_masks(cnt, max_atom_num), state=atoms)
+                # (piece_draw keeps the end token out of the first step)
+                shaping.update(allowed=ops.pack_allowed(self._atoms_allowed(cnt, max_atom_num)), state=atoms)
         for t in range(max_pos):
             emb = self.piece_embedding(cur).contiguous()
             hip.gemm(B, 3 * H, E, emb, E, 1, w_ih, 1, E, gi, 3 * H, bias=rnn.bias_ih_l0)
