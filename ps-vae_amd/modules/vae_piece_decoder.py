@@ -284,9 +284,12 @@ class VAEPieceDecoder(nn.Module):
 
     def piece_log_prob(self, z_vecs, pieces, temperature=1.0, shaping=None, max_atom_num=None, piece_atom_counts=None):
         """Log-probability of every piece of given sequences under the distribution that sample_pieces_batch draws from with the
-        same temperature and shaping - what a policy gradient on sampled molecules needs, differentiable in the latents and the
-        parameters.  pieces [B, S] int64 as in training: <s>, the pieces, the end token, then <pad>.  Returns [B, S - 1]
-        float32, 0 at padding."""
+        same temperature and shaping, differentiable in the latents and the parameters.  pieces [B, S] int64 as in training: <s>, the
+        pieces, the end token, then <pad>.  Returns [B, S - 1] float32, 0 at padding.
+
+        For a policy gradient on sampled molecules the pieces are <s> and the tokens as drawn (sample_pieces_batch with
+        return_draws): a molecule that ran out of positions, or grew too large, ended with a piece and not with an end token.
+        Where fit_atoms leaves no piece for the first position the loop takes the end token for certain: 0."""
         shaping = dict(shaping or {})
         cnt = self.tokenizer.piece_atom_counts() if piece_atom_counts is None else piece_atom_counts
         cnt = torch.as_tensor(cnt, dtype=torch.int32, device=pieces.device)
@@ -295,8 +298,9 @@ class VAEPieceDecoder(nn.Module):
             raise ValueError('fit_atoms needs max_atom_num')
         # row 0 is the first position's; behind the rows for the numbers of atoms one for none at a later position (after pieces without atoms)
         allowed = self._atoms_allowed(cnt, max_atom_num if fit else None)
-        last, later = allowed.shape[0] - 1, allowed[:1].clone()
-        allowed[0, self.tokenizer.end_idx()] = False
+        last, later, end = allowed.shape[0] - 1, allowed[:1].clone(), self.tokenizer.end_idx()
+        allowed[0, end] = False
+        allowed[0, end] = ~allowed[0].any()
         masks = ops.pack_allowed(torch.cat([allowed, later]))
         gold = pieces[:, 1:].contiguous()
         atoms = cnt[gold]
@@ -311,7 +315,7 @@ class VAEPieceDecoder(nn.Module):
 
     @torch.no_grad()
     def sample_pieces_batch(self, z, max_atom_num, temperature, uniforms=None, piece_atom_counts=None,
-                            generator=None, shaping=None):
+                            generator=None, shaping=None, return_draws=False):
         """The piece sampling loop of `inference` (:134-158) for a batch of latents: every step
         is one GRU cell over all still-active molecules (two GEMMs + the fused gate kernel),
         the vocabulary projection, the pad / first-step end masks, softmax(logits / T) and one
@@ -325,7 +329,12 @@ class VAEPieceDecoder(nn.Module):
         shaping: what else is done to the logits before the draw (the reference does nothing): a dict of repetition,
         presence, frequency (penalties for the pieces that a molecule already has) and bias, as ops.shape_logits takes
         them, and fit_atoms=True: only pieces that keep the molecule within max_atom_num atoms, so that none is
-        sampled only to be dropped."""
+        dropped for its size (the last of max_pos pieces still is).
+
+        return_draws: also returns the tokens as they were drawn, [B, max_pos] int64 padded with pad_idx, and how many of them
+        a molecule has, [B] int64: its pieces and then the draw that ended it - the end token, or the piece that is dropped.
+        This is what piece_log_prob scores: torch.cat([<s>, draws], 1).
+        """
         dev = self.W_mean.weight.device
         tok = self.tokenizer
         z = z.to(dev).float().reshape(-1, self.latent_dim)
@@ -377,7 +386,8 @@ class VAEPieceDecoder(nn.Module):
         length = length.to(torch.int64)
         lengths = (length - 1).clamp(min=0)
         keep = torch.arange(max_pos, device=dev)[None, :] < lengths[:, None]
-        return torch.where(keep, out, torch.full_like(out, pad)), lengths
+        ids = torch.where(keep, out, torch.full_like(out, pad))
+        return (ids, lengths, out, length) if return_draws else (ids, lengths)
 
     @torch.no_grad()
     def infer_links_batch(self, z, x, x_pieces, x_pos, node_off, csr_in, frag, add_edge_th):

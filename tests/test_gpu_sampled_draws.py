@@ -1,5 +1,5 @@
-"""The piece sampling loop under penalties, a bias and the atom budget, followed draw by draw with the float64 oracle, and given
-sequences scored by piece_log_prob under the same rules."""
+"""The piece sampling loop under penalties, a bias and the atom budget, followed draw by draw with the float64 oracle; and the draws it returns scored
+by piece_log_prob: exactly the tokens that were drawn, for every reason that a molecule can stop for."""
 import numpy as np
 import pytest
 import torch
@@ -117,6 +117,9 @@ def scored(dec, tok, z, draws, counts, temperature, shaping, budget, monkeypatch
                 allowed = cnt + (cnt[past].sum() if past else 0) <= budget
             allowed[tok.end_idx()] = t > 0
             allowed[tok.pad_idx()] = False
+            if not allowed.any():                      # the loop has no choice but the end token
+                assert seq[t] == tok.end_idx() and got[b, t] == 0.0
+                continue
             assert allowed[seq[t]], (b, t)
             s = shaping or {}
             y, slope, scale = shaping_ref.shaped_row(rows[b, t], past, f32(s.get('repetition', 1.)), f32(s.get('presence', 0.)),
@@ -147,3 +150,35 @@ def test_pieces_without_atoms(fit, monkeypatch):
         pieces = pieces[n1 > 0]
         assert pieces.shape[0] > 10
         scored(dec, tok, z[n1 > 0], pieces[:, 1:], n1[n1 > 0] + 1, 1.0, dict(fit_atoms=fit), 500, monkeypatch, atoms=cnt)
+
+
+@pytest.mark.parametrize('max_pos,budget,shaping', [(3, 200, None), (12, 9, None), (12, 9, dict(presence=0.4)), (4, 30, dict(fit_atoms=True, repetition=1.3)),
+                                                    (12, 20, dict(fit_atoms=True)), (5, 0, dict(fit_atoms=True))])
+def test_the_draws_are_what_is_scored(max_pos, budget, shaping, monkeypatch):
+    B, temperature = 80, 0.9
+    dec, tok, z, u = setup(B, 31, max_pos)
+    ids, lengths = dec.sample_pieces_batch(z, budget, temperature, uniforms=u, shaping=shaping)
+    steps = Steps(monkeypatch)
+    again, n, draws, counts = dec.sample_pieces_batch(z, budget, temperature, uniforms=u, shaping=shaping, return_draws=True)
+    monkeypatch.undo()
+    assert torch.equal(ids, again) and torch.equal(lengths, n)
+    assert draws.shape == (B, max_pos) and draws.dtype == torch.int64 and counts.dtype == torch.int64 and torch.equal((counts - 1).clamp(min=0), lengths)
+    taken = torch.stack(steps.picks, 1)
+    assert torch.equal(draws[:, :taken.shape[1]], taken)
+    # every reason to stop that these sizes allow is there, and the last draw is the one that was made
+    cnt = np.asarray(tok.piece_atom_counts())
+    reasons = set()
+    for b in range(B):
+        seq = draws[b, :int(counts[b])].tolist()
+        assert draws[b, int(counts[b]):].eq(tok.pad_idx()).all() and seq[:-1] == ids[b, :int(lengths[b])].tolist()
+        reasons.add('end' if seq[-1] == tok.end_idx() else 'atoms' if cnt[seq].sum() > budget else 'positions')
+    if budget == 200:
+        assert 'positions' in reasons
+    if budget == 9:
+        assert 'atoms' in reasons
+    if shaping and 'fit_atoms' in shaping:
+        assert 'atoms' not in reasons
+    if budget == 30:
+        assert 'positions' in reasons                # a piece that fits is dropped at the last position all the same
+    lp = scored(dec, tok, z, draws, counts, temperature, shaping, budget, monkeypatch)
+    assert bool(torch.isfinite(lp).all())
