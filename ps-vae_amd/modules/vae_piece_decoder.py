@@ -364,9 +364,12 @@ class VAEPieceDecoder(nn.Module):
         cnt = cnt.to(torch.int32)
         if shaping is not None:
             shaping = dict(shaping)
-            if {'repetition', 'presence', 'frequency'} & shaping.keys():
+            penalties, fit = {'repetition', 'presence', 'frequency'} & shaping.keys(), shaping.pop('fit_atoms', False)
+            if (penalties and {'history', 'history_len'} & shaping.keys()) or (fit and {'allowed', 'state'} & shaping.keys()):
+                raise ValueError('shaping: penalties are for the pieces drawn here, and fit_atoms brings its own masks')
+            if penalties:
                 shaping.update(history=out, history_len=length)
-            if shaping.pop('fit_atoms', False):
+            if fit:
                 # (piece_draw keeps the end token out of the first step)
                 shaping.update(allowed=ops.pack_allowed(self._atoms_allowed(cnt, max_atom_num)), state=atoms)
         for t in range(max_pos):

@@ -182,3 +182,18 @@ def test_the_draws_are_what_is_scored(max_pos, budget, shaping, monkeypatch):
         assert 'positions' in reasons                # a piece that fits is dropped at the last position all the same
     lp = scored(dec, tok, z, draws, counts, temperature, shaping, budget, monkeypatch)
     assert bool(torch.isfinite(lp).all())
+
+
+def test_options_that_would_be_overridden_are_refused():
+    from ps_vae_amd import ops
+    dec, tok, z, u = setup(4, 51, 6)
+    masks = ops.pack_allowed(torch.ones(1, tok.num_piece_type(), dtype=torch.bool, device=dev()))
+    past = torch.zeros(4, 3, dtype=torch.int64, device=dev())
+    for shaping in (dict(fit_atoms=True, allowed=masks), dict(presence=0.5, history=past),
+                    dict(presence=0.5, history_len=torch.zeros(4, dtype=torch.int32, device=dev()))):
+        with pytest.raises(ValueError):
+            dec.sample_pieces_batch(z, 20, 1.0, uniforms=u, shaping=shaping)
+    ids, _ = dec.sample_pieces_batch(z, 20, 1.0, uniforms=u, shaping=dict(allowed=masks))     # alone it says what it does
+    assert torch.equal(ids, dec.sample_pieces_batch(z, 20, 1.0, uniforms=u)[0])
+    with pytest.raises(ValueError, match='max_atom_num'):
+        dec.piece_log_prob(z, past, shaping=dict(fit_atoms=True))
