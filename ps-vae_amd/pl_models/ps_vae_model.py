@@ -208,15 +208,15 @@ class PSVAEModel(nn.Module):
     def inference_single_z(self, z, max_atom_num, add_edge_th, temperature):
         return self.decoder.inference(z, max_atom_num, add_edge_th, temperature)
 
-    def inference_batch_z(self, zs, max_atom_num, add_edge_th, temperature, constraint_mol=None):
+    def inference_batch_z(self, zs, max_atom_num, add_edge_th, temperature, constraint_mol=None, shaping=None):
         """The reference loops inference_single_z over the latents (:139-141, "not accelerating,
         just a loop"); here the whole batch goes through sampling, link prediction and greedy
         assembly at once.  Returns one atoms / bonds dict per latent (see
-        VAEPieceDecoder.inference_batch)."""
+        VAEPieceDecoder.inference_batch); shaping: see VAEPieceDecoder.sample_pieces_batch."""
         if constraint_mol is not None:
             raise NotImplementedError('constrained generation (inference_constraint) is outside the accelerated path')
         zs = torch.stack(list(zs)) if not torch.is_tensor(zs) else zs
-        mols, _ = self.decoder.inference_batch(zs, max_atom_num, add_edge_th, temperature)
+        mols, _ = self.decoder.inference_batch(zs, max_atom_num, add_edge_th, temperature, shaping=shaping)
         return mols
 
     def predict_props(self, z):
