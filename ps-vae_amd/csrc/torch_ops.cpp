@@ -10,10 +10,10 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
-#include <algorithm>
 #include <initializer_list>
 #include <map>
 #include <mutex>
@@ -631,20 +631,21 @@ psvae_shaping shaping_of(const ShapingArgs &a, const char *fn) {
     "Tensor logits, Tensor? history, Tensor? history_len, Tensor? repetition, Tensor? presence, Tensor? frequency, " \
     "Tensor? temperature, float[] scalars, Tensor? bias, Tensor? allowed, Tensor? state"
 
-// No operator here has a forward-mode derivative: a tangent on an operand is an error, for the result would come back without one.
-void no_tangents(const char *fn, std::initializer_list<const Tensor *> operands) {
-    for (const Tensor *t : operands)
-        TORCH_CHECK(t == nullptr || !t->_fw_grad(0).defined(), fn, ": forward-mode derivatives are not implemented");
-}
+// No operator here has a forward-mode derivative: a tangent on an operand is an error, for the result would come back without one.  (Tangents
+// live inside a level of forward mode alone: outside, one question for the level takes the place of one for each operand.)
+bool in_forward_mode() { return torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr; }
+void no_tangent(const char *fn, const Tensor &t) { TORCH_CHECK(!t._fw_grad(0).defined(), fn, ": forward-mode derivatives are not implemented"); }
 bool wants_gradient(const Tensor &t) { return at::GradMode::is_enabled() && t.requires_grad(); }
-bool wants_gradient(at::TensorList ts) { return std::any_of(ts.begin(), ts.end(), [](const Tensor &t) { return wants_gradient(t); }); }
 
 // What is asked of a call's floating operands: only the logits have a gradient, in reverse mode.
 void check_operands(const char *fn, const Tensor &logits, std::initializer_list<const Tensor *> data) {
-    no_tangents(fn, {&logits});
-    no_tangents(fn, data);
-    for (const Tensor *t : data)
-        TORCH_CHECK(t == nullptr || !wants_gradient(*t), fn, ": penalties, temperature and bias are data: none of them gets a gradient");
+    const bool forward_mode = in_forward_mode();
+    if (forward_mode) no_tangent(fn, logits);
+    for (const Tensor *t : data) {
+        if (t == nullptr) continue;
+        if (forward_mode) no_tangent(fn, *t);
+        TORCH_CHECK(!wants_gradient(*t), fn, ": penalties, temperature and bias are data: none of them gets a gradient");
+    }
 }
 #define PSVAE_CHECK_OPERANDS(fn) check_operands(fn, logits, {p(repetition), p(presence), p(frequency), p(temperature), p(bias)})
 
@@ -664,7 +665,7 @@ Tensor shape_logits_forward(PSVAE_SHAPING_PARAMS) {
 Tensor shape_logits_backward(const Tensor &g, PSVAE_SHAPING_PARAMS) {
     PSVAE_ON_DEVICE("psvae::shape_logits_backward", p(g), PSVAE_SHAPING_TENSORS);
     const char *fn = "psvae_shape_logits_bwd";
-    no_tangents(fn, {p(g)});
+    if (in_forward_mode()) no_tangent(fn, g);
     const psvae_shaping s = shaping_of(PSVAE_SHAPING_ARGS, fn);
     TORCH_CHECK(g.sizes() == logits.sizes() && g.scalar_type() == logits.scalar_type(), fn, ": the gradient has the logits' shape and type");
     const Tensor gc = s.V == 1 || g.stride(-1) == 1 ? g : g.contiguous();
@@ -698,7 +699,7 @@ std::tuple<Tensor, Tensor> shaped_log_prob_forward(const Tensor &tokens, PSVAE_S
 Tensor shaped_log_prob_backward(const Tensor &g, const Tensor &stats, const Tensor &tokens, PSVAE_SHAPING_PARAMS) {
     PSVAE_ON_DEVICE("psvae::shaped_log_prob_backward", p(g), p(stats), p(tokens), PSVAE_SHAPING_TENSORS);
     const char *fn = "psvae_shaped_log_prob_bwd";
-    no_tangents(fn, {p(g)});
+    if (in_forward_mode()) no_tangent(fn, g);
     const psvae_shaping s = shaping_of(PSVAE_SHAPING_ARGS, fn);
     const int64_t *tok = row_tokens(tokens, logits, fn);
     const int64_t rows = (int64_t)s.B * s.T;
@@ -802,14 +803,17 @@ struct TensorList {
     std::vector<const void *> ptr;
     std::vector<int64_t> numel;
     std::vector<int32_t> types;
+    bool followed = false;          // by autograd: some tensor requires a gradient while gradients are recorded
 };
 TensorList list_of(at::TensorList ts, c10::Device device, const char *fn) {
     TensorList l;
+    const bool forward_mode = in_forward_mode(), recorded = at::GradMode::is_enabled();
     l.ptr.reserve(ts.size()), l.numel.reserve(ts.size()), l.types.reserve(ts.size());
     for (const Tensor &t : ts) {
         TORCH_CHECK(t.is_cuda(), fn, ": psvae operators need GPU tensors (there is no CPU fallback)");
         TORCH_CHECK(t.device() == device, fn, ": tensors on different devices (", device, " and ", t.device(), ")");
-        no_tangents(fn, {&t});
+        if (forward_mode) no_tangent(fn, t);
+        l.followed |= recorded && t.requires_grad();
         TORCH_CHECK(t.layout() == at::kStrided && t.is_non_overlapping_and_dense(), fn,
                     ": a gradient must be dense, each of its elements in a place of its own");
         l.ptr.push_back(t.const_data_ptr()), l.numel.push_back(t.numel()), l.types.push_back(elem_type(t, fn));
@@ -827,17 +831,17 @@ Tensor grad_norm(at::TensorList grads) {
     const size_t nbytes = psvae_grad_norm_workspace_bytes(n);
     Tensor hold = scratch(nbytes, norm);
     check(psvae_grad_norm(n, l.ptr.data(), l.numel.data(), l.types.data(), norm.data_ptr<float>(), hold.data_ptr(), nbytes, cur_stream(norm)), fn);
-    return wants_gradient(grads) ? end_of_graph(norm, "psvae_grad_norm: the norm cannot be differentiated") : norm;
+    return l.followed ? end_of_graph(norm, "psvae_grad_norm: the norm cannot be differentiated") : norm;
 }
 
 Tensor clip_grads(at::TensorList grads, double max_norm, at::TensorList out) {
     const char *fn = "psvae_clip_grads";
     TORCH_CHECK(!grads.empty() && out.size() == grads.size(), fn, ": one output for each of at least one gradient");
-    // (written through its pointer, a leaf would change behind autograd's back and a result of a graph would keep its old derivative)
-    TORCH_CHECK(!wants_gradient(grads) && !wants_gradient(out), fn,
-                ": a tensor requires a gradient, and scaling cannot be differentiated: call it under torch.no_grad()");
     c10::DeviceGuard guard(same_device(fn, {&grads[0]}));
     const TensorList l = list_of(grads, grads[0].device(), fn), o = list_of(out, grads[0].device(), fn);
+    // (written through its pointer, a leaf would change behind autograd's back and a result of a graph would keep its old derivative)
+    TORCH_CHECK(!l.followed && !o.followed, fn,
+                ": a tensor requires a gradient, and scaling cannot be differentiated: call it under torch.no_grad()");
     const int n = (int)grads.size();
     for (int i = 0; i < n; ++i)
         TORCH_CHECK(out[i].numel() == grads[i].numel() &&
