@@ -852,8 +852,13 @@ __global__ __launch_bounds__(NT) void shape_run_bwd_kernel(Args a, const T *__re
 // ---- log_prob.  Measured, 4000 rows of 32768 bf16 with histories of up to 500, a bias and masks: forward 84 us (262 MB; 50 us, 5.2 TB/s, with neither
 // bias nor history: the bias costs 15, its 4 bytes an element coming from L2, the look back 11), backward 99.6 us (524 MB: 5.3 TB/s).
 // Streamed stores took the backward from 163 to 128 us, reading the rows from the end 154 to 128, whole lines (Stage) 122 to 101.
-// Sums are 32-bit: a lane's at most 128 terms of a run in a chain (rescaled where its maximum grows), 6 levels over the wave, 4
-// waves, then the row's runs: the relative error stays below (128 + 10 + runs) * 2^-24 and is far below it on average.
+// Sums are 32-bit.  With u = 2^-24, the sum's relative error is at most
+//     (3 ln V + 2) u   from the exponentials: three rounded factors in each argument t = y - m, which weighted by the terms themselves averages at
+//                      most ln V (what a lane's maximum moved by on the way counts as part of t), and the unit's 1 ulp,
+//     3 u              for each rescaling of a partial sum: a lane's steps (8 of 16 elements in a run of 32768) and entries of the list of seen ids
+//                      (at most 4096 over 256 threads: 16), then its wave, the workgroup and the row,
+//     u                for each addition: 128 terms and 16 entries in a lane's chain, 6 levels over the wave, 4 waves, runs / 64 + 6 over the row's runs:
+// under 290 u + u runs / 64 for a row of 32768, and far below it on average.
 template <typename T, int N>
 __global__ __launch_bounds__(NT) void log_prob_rows_kernel(Args a, const int64_t *__restrict__ tokens, float *__restrict__ lp,
                                                            float2 *__restrict__ stats) {
