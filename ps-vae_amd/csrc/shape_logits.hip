@@ -1227,9 +1227,11 @@ Cut cut_of(const psvae_shaping *s) {
         c.blocks = (R + WAVES - 1) / WAVES;
         return c;
     }
-    // The longest runs that leave 960 workgroups, close to 4 for each compute unit (a run pays for its walk through the history once: 250 rows
-    // of 100003 in 4 runs each 44 us, in 5 47, in 8 51); down
-    // to 2048 elements, in smaller steps, where rows are few.  A long history's list of seen ids has to fit LDS: at most 4096 of them.
+    // The longest runs that leave 960 workgroups: a run pays for its walk through the history once, and 4 workgroups for each compute unit, 1024,
+    // are in flight at a time.  The number of runs being rounded up, 960 seldom comes to more than 1024, and aiming at 1024 does: draws of 120, 200
+    // and 250 rows of 100003 take 30, 38 and 44 us, and 33, 43 and 46; of 32003 16, 20 and 21, and 16, 24 and 24.  The other way round at 64 rows
+    // (32003: 14.4 and 13.1 us; 131072: 23 and 22); under 32 rows and over 330 there is no difference.  Down to 2048 elements, in smaller steps, where
+    // rows are few.  A long history's list of seen ids has to fit LDS: at most 4096 of them.
     const int longest = s->history != nullptr && s->L > 4096 ? 4096 : RUN_MAX;
     long long runs = std::max<long long>(psvae_cdiv(s->V, longest), std::min<long long>(psvae_cdiv(s->V, 2048), (960 + R - 1) / std::max<long long>(R, 1)));
     c.run = psvae_cdiv(psvae_cdiv(s->V, runs), 1024) * 1024;
