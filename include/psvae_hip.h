@@ -546,7 +546,7 @@ typedef struct psvae_shaping {
     int64_t ld_b, ld_t;
     const int64_t *history;         /* [B, L], rows ld_history apart; null: no penalties         */
     int64_t ld_history;
-    int L;
+    int L;                          /* room: over 4096, wide rows are cut into shorter runs (slower) */
     const int32_t *history_len;     /* [B], or [B, T] when len_per_row; null: L                  */
     int len_per_row;
     const float *repetition_rows, *presence_rows, *frequency_rows, *temperature_rows;   /* [B], or null: */

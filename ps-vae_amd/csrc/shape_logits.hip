@@ -7,7 +7,8 @@
 //     draw:  min(#{i : cdf_i <= u cdf_last}, last i of positive probability),  cdf the running sum of exp(y - m) in index order
 //
 // Bound: one read of the logits (and one write) at large sizes, launches at small ones, with 8 to 14 vector instructions an element in
-// between that have to stay under the time of the loads; the draw, whose 25 of 38 are 64-bit, is bound by them.
+// between that have to stay under the time of the loads (shape of wide rows: the vector unit 21 % busy; log_prob both ways: 80 %, so
+// this bounds it as much as the loads); the draw, whose 25 of 38 are 64-bit, is bound by them (77 %).
 //
 // Rows of at most 1024 logits: one wave each (Narrow).  Wider rows are cut into runs of up to 32768 elements, a workgroup each, whose
 // waves stream through it in steps of 512 or 1024 elements (`stream`).
@@ -1231,7 +1232,12 @@ Cut cut_of(const psvae_shaping *s) {
     // are in flight at a time.  The number of runs being rounded up, 960 seldom comes to more than 1024, and aiming at 1024 does: draws of 120, 200
     // and 250 rows of 100003 take 30, 38 and 44 us, and 33, 43 and 46; of 32003 16, 20 and 21, and 16, 24 and 24.  The other way round at 64 rows
     // (32003: 14.4 and 13.1 us; 131072: 23 and 22); under 32 rows and over 330 there is no difference.  Down to 2048 elements, in smaller steps, where
-    // rows are few.  A long history's list of seen ids has to fit LDS: at most 4096 of them.
+    // rows are few.  A long history's list of seen ids has to fit LDS: at most 4096 of them.  So with ROOM for more (L; how many are in use is only
+    // known on the device) runs have at most 4096 elements, and every one of them walks the history - twice, where more than 4096 ids are in use, which
+    // are then not kept in between: rows * (V / 4096) * 16 * (ids in use) bytes, mostly from L2.  250 rows of 100003 f16, shape / log_prob / draw_run:
+    //     500 ids in use, room for 4096: 28 / 22 / 35 us;  room for 4097, or 65536: 42 / 41 / 47
+    //     4096 ids: 43 / 31 / 44;  4097: 80 / 72 / 81;  8192: 118 / 104 / 110;  65536: 694 / 566 / 573
+    // (16 rows or fewer have short runs anyway: no difference between a room of 4096 and one of 65536.)
     const int longest = s->history != nullptr && s->L > 4096 ? 4096 : RUN_MAX;
     long long runs = std::max<long long>(psvae_cdiv(s->V, longest), std::min<long long>(psvae_cdiv(s->V, 2048), (960 + R - 1) / std::max<long long>(R, 1)));
     c.run = psvae_cdiv(psvae_cdiv(s->V, runs), 1024) * 1024;
