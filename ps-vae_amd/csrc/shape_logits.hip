@@ -1230,8 +1230,8 @@ Cut cut_of(const psvae_shaping *s) {
     }
     // The longest runs that leave 960 workgroups: a run pays for its walk through the history once, and 4 workgroups for each compute unit, 1024,
     // are in flight at a time.  The number of runs being rounded up, 960 seldom comes to more than 1024, and aiming at 1024 does: draws of 120, 200
-    // and 250 rows of 100003 take 30, 38 and 44 us, and 33, 43 and 46; of 32003 16, 20 and 21, and 16, 24 and 24.  The other way round at 64 rows
-    // (32003: 14.4 and 13.1 us; 131072: 23 and 22); under 32 rows and over 330 there is no difference.  Down to 2048 elements, in smaller steps, where
+    // and 250 rows of 100003 take 30, 38 and 44 us, and 33, 43 and 46; of 32003 16, 20 and 21, and 16, 24 and 24.  The other way round at
+    // 64 rows (32003: 14.4 and 13.1 us; 131072: 23 and 22); 16 rows or fewer and 700 or more show no difference.  Down to 2048 elements, in smaller steps, where
     // rows are few.  A long history's list of seen ids has to fit LDS: at most 4096 of them.  So with ROOM for more (L; how many are in use is only
     // known on the device) runs have at most 4096 elements, and every one of them walks the history - twice, where more than 4096 ids are in use, which
     // are then not kept in between: rows * (V / 4096) * 16 * (ids in use) bytes, mostly from L2.  250 rows of 100003 f16, shape / log_prob / draw_run:

@@ -1058,8 +1058,9 @@ def shape_logits(logits, *, history=None, history_len=None, repetition=None, pre
         y_i = (a_i + bias_i) / temperature   where the row's mask allows i, else -inf
 
     history int64 [B, L] (ids outside the vocabulary count for nothing: padding may be negative); history_len int32 [B] or
-    [B, T] (None: L).  Over many wide rows an L above 4096 costs time whatever history_len says: pass the part that is in use.  repetition, presence, frequency, temperature: a number or float32 [B], repetition
-    and temperature in 2^-126 .. 2^126.  bias float32 [V] or [B, V].
+    [B, T] (None: L).  Over many wide rows an L above 4096 costs time whatever history_len says: pass the part that is in use.
+    repetition, presence, frequency, temperature: a number or float32 [B], repetition and temperature in 2^-126 .. 2^126.
+    bias float32 [V] or [B, V].
     allowed: a table of masks (pack_allowed); state int32 [B] or [B, T]: the table's row for each row of logits - negative: nothing is
     forbidden, past the table: everything is; None: the table has one row for all, or one per sequence.
 

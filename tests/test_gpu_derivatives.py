@@ -168,3 +168,18 @@ def test_data_operands_that_want_a_gradient():
                 assert torch.equal(a, b), name
     with torch.no_grad():
         assert torch.equal(ops.shape_logits(c['x'], bias=torch.nn.Parameter(c['bias'])), ops.shape_logits(c['x'], bias=c['bias']))
+
+
+def test_function_transforms_are_errors():
+    """torch.func's derivatives wrap their tensors: neither comes back with a result that lacks one."""
+    from ps_vae_amd import optim
+    c = inputs()
+    ones = torch.ones_like(c['x'])
+    single = {name: (lambda x, call=call: call(x)[1] if isinstance(call(x), tuple) else call(x)) for name, call in calls(c).items()}
+    single['grad_norm'] = lambda x: optim.grad_norm([x])
+    for f in single.values():
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(f, (c['x'],), (ones,))
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda x, f=f: f(x).sum())(c['x'])
+        assert bool(torch.isfinite(f(c['x'])).all())
